@@ -1035,6 +1035,7 @@ paged_attention_merge_kernel(const float* __restrict__ partial, T* __restrict__ 
 
 }  // namespace mxb
 #include "attention_decode_project.cuh"
+#include "attention_decode_quantized.cuh"
 namespace mxb {
 
 // What follows the attention kernel of a decode step: the merge of the partial
@@ -1291,6 +1292,56 @@ MXB_API int mxb_paged_attention_decode_project(const void* q, const void* cache,
              heads, kv_heads, page_tokens, num_pages, max_splits, window, chunk, keep, scale, status, stream, project
   return head_dim == 64 ? launch_decode_mma<64>(ARGS) : launch_decode_mma<128>(ARGS);
 #undef ARGS
+}
+
+// Whether the decode kernels over a cache in 8 bits take this head layout.
+MXB_API int mxb_paged_attention_decode_quantized_supported(int head_dim, int heads, int kv_heads, int dtype) {
+  return head_dim > 0 && head_dim <= 256 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && (dtype == kF32 || dtype == kBF16) ? 1 : 0;
+}
+
+// mxb_paged_attention_decode over a cache in 8 bits: codes [pages, 2, kv_heads,
+// page_tokens, head_dim] and scales [pages, 2, kv_heads, page_tokens]. With w
+// (bfloat16 heads of 64 or 128 values, up to 64 tokens) the partial results are
+// put together and projected by one kernel, as mxb_paged_attention_decode_project does.
+MXB_API int mxb_paged_attention_decode_quantized(const void* q, const void* codes, const float* scales, int kind, void* out, float* partial,
+                                                 const int* block_tables, int max_pages, const int* row_token, const int* row_request,
+                                                 const int* positions, int rows, int tokens, int heads, int kv_heads, int head_dim,
+                                                 int page_tokens, int num_pages, int max_splits, int window, int chunk, int keep,
+                                                 float scale, int dtype, const void* w, long long ldw, int hidden, float* summands,
+                                                 const void* gate, long long gate_stride, float softcap, int has_sink, float sink_score,
+                                                 const float* sink_heads, const float* bias_table, int bias_far, int* status,
+                                                 cudaStream_t stream) {
+  if (rows <= 0) return 0;
+  if (!mxb_paged_attention_decode_quantized_supported(head_dim, heads, kv_heads, dtype) || max_splits <= 0 || page_tokens <= 0 ||
+      num_pages <= 0 || rows > 65535 || (kind != kCodesE4M3 && kind != kCodesInt8) || (bias_table != nullptr && bias_far < 0) ||
+      static_cast<long long>(num_pages) * 2 * kv_heads * page_tokens > 0x7fffffffLL)
+    return static_cast<int>(cudaErrorInvalidValue);
+  if (w != nullptr && (dtype != kBF16 || hidden <= 0 || !decode_project_takes(head_dim, tokens, w, ldw)))
+    return static_cast<int>(cudaErrorInvalidValue);
+  const QuantizedDecode args = {q, static_cast<const uint8_t*>(codes), scales, partial, block_tables, max_pages, row_token, row_request,
+                                positions, heads, kv_heads, head_dim, page_tokens, num_pages, window, chunk, keep, scale, softcap,
+                                ScoreBias{bias_table, bias_far}, status};
+  const int slots = quantized_slots(rows * kv_heads, max_splits);
+  const cudaError_t e = dtype == kF32 ? launch_quantized_decode<float>(args, kind, rows, slots, stream)
+                                      : launch_quantized_decode<__nv_bfloat16>(args, kind, rows, slots, stream);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (w != nullptr) {
+    auto project = head_dim == 64 ? launch_merge_project<64> : launch_merge_project<128>;
+    return static_cast<int>(project(partial, static_cast<const __nv_bfloat16*>(w), ldw, summands, row_token, positions, rows, tokens,
+                                    heads, hidden, max_splits, window, chunk, keep, slots, kSplitKeys, kDecodeMinusHuge,
+                                    static_cast<const __nv_bfloat16*>(gate), gate_stride, has_sink, sink_score, sink_heads, status,
+                                    stream));
+  }
+  auto merge = [&](auto* target, const auto* gates) {
+    using T = std::remove_pointer_t<decltype(target)>;
+    return static_cast<int>(launch_chained(paged_attention_merge_kernel<T>, dim3(rows, heads),
+                                           dim3(head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256)), 0, stream,
+                                           static_cast<const float*>(partial), target, row_token, positions, rows, heads, head_dim,
+                                           max_splits, window, chunk, keep, slots, gates, gate_stride, has_sink, sink_score,
+                                           sink_heads, status));
+  };
+  if (dtype == kF32) return merge(static_cast<float*>(out), static_cast<const float*>(gate));
+  return merge(static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(gate));
 }
 
 // ---------------------------------------------------------------------------

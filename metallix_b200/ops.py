@@ -90,6 +90,12 @@ _SIGNATURES = {
     "mxb_plain_activation": [_P, _P, _L, _I, _I, _P],
     "mxb_paged_attention_decode": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
                                    _F, _I, _P, _L, _F, _I, _F, _P, _P, _I, _P, _P],
+    "mxb_paged_attention_decode_quantized_supported": [_I, _I, _I, _I],
+    "mxb_paged_attention_decode_quantized": [_P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
+                                             _F, _I, _P, _L, _I, _P, _P, _L, _F, _I, _F, _P, _P, _I, _P, _P],
+    "mxb_store_quantized": [_P, _P, _P, _L, _L, _L, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _I, _I, _I, _I, _I,
+                            _F, _I, _P, _I, _P, _P],
+    "mxb_read_cache": [_P, _P, _I, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "mxb_postnorm_add_rmsnorm": [_P, _P, _I, _I, _P, _F, _P, _I, _P, _F, _I, _I, _P],
     "mxb_sigmoid_gate": [_P, _P, _P, _L, _L, _L, _I, _I, _I, _P],
     "mxb_softcap": [_P, _F, _L, _P],
@@ -1290,9 +1296,93 @@ def copy_units_by_host(copies) -> None:
         _call("mxb_copy_spans", (ctypes.c_longlong * len(spans))(*spans), len(spans) // 5, _stream())
 
 
+# ------------------------------------------------------------ caches in 8 bits
+_CODE_KINDS = {torch.float8_e4m3fn: 0, torch.int8: 1}
+CODE_DTYPES = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}
+
+
+class QuantizedPool:
+    """One cache entry's pages held in 8 bits: ``codes``
+    ``[pages, 2, kv_heads, page_tokens, head_dim]`` (float8_e4m3fn or int8) and
+    ``scales`` ``[pages, 2, kv_heads, page_tokens]`` (float32). Row x is kept as
+    scale = max |x| / limit in float32 (limit 448 for e4m3, 127 for int8) and
+    the codes nearest to the exact quotients x / scale (of two equally near the
+    even one); it stands for code * scale. A row of zeros has scale 0. A row
+    with an infinity or a NaN has scale NaN: it stands for NaN throughout.
+
+    ``write_cache``, ``qk_norm_rope_cache``, ``paged_attention_decode`` and
+    ``paged_attention_decode_project`` take one wherever they take a cache in the
+    compute type; ``read_cache`` turns pages back into such a cache, which the
+    other attention kernels read."""
+
+    __slots__ = ("codes", "scales")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        _check(codes, "codes", tuple(_CODE_KINDS), 5)
+        _check(scales, "scales", (torch.float32,), 4)
+        _need(codes.shape[1] == 2, "codes must be [pages, 2, kv_heads, page_tokens, head_dim]")
+        _need(scales.shape == codes.shape[:4], "one scale per row: scales must be [pages, 2, kv_heads, page_tokens]")
+        _need(scales.device == codes.device, "codes and scales are on different devices")
+        _need(scales.numel() < 1 << 31, f"a pool of {scales.numel()} rows: the kernels count rows in 31 bits")
+        self.codes, self.scales = codes, scales
+
+    @classmethod
+    def zeros(cls, pages: int, kv_heads: int, page_tokens: int, head_dim: int, codes: str = "fp8",
+              device="cuda:0") -> "QuantizedPool":
+        _need(codes in CODE_DTYPES, f"codes must be one of {sorted(CODE_DTYPES)}, got {codes!r}")
+        shape = (pages, 2, kv_heads, page_tokens, head_dim)
+        return cls(torch.zeros(shape, dtype=CODE_DTYPES[codes], device=device),
+                   torch.zeros(shape[:4], dtype=torch.float32, device=device))
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def kind(self) -> int:
+        return _CODE_KINDS[self.codes.dtype]
+
+
+def _on_current_device(**tensors) -> None:
+    """The kernels run on the current device's current stream: everything has to be there."""
+    current = torch.cuda.current_device()
+    for name, tensor in tensors.items():
+        _need(tensor is None or tensor.device.index == current,
+              f"{name} is on another device than the current one (cuda:{current})")
+
+
+def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tensor, row_request: torch.Tensor,
+               first: torch.Tensor, last: torch.Tensor, window: int = 0, chunk: int = 0, keep: int = 0) -> torch.Tensor:
+    """Pages of a quantized pool back into the compute type: for every i the
+    pages of row ``row_request[i]`` of ``block_tables`` that queries from
+    position ``first[i]`` on see (``window``, ``chunk`` and ``keep`` as the
+    attention kernels take them), up to position ``last[i]``. ``out`` (float32
+    or bfloat16) has the pool's shape: a page keeps its number, so the same
+    block tables serve it; rows that are not read stay as they are. A negative
+    ``last`` reads nothing."""
+    _need(isinstance(pool, QuantizedPool), "pool must be a QuantizedPool")
+    _check(out, "out", tuple(_CODES), 5)
+    _need(out.shape == pool.shape, "out must have the pool's shape")
+    _check(block_tables, "block_tables", (torch.int32,), 2)
+    for name, tensor in (("row_request", row_request), ("first", first), ("last", last)):
+        _check(tensor, name, (torch.int32,), 1)
+    rows = row_request.numel()
+    _need(first.numel() == rows and last.numel() == rows, "row lists differ in length")
+    _need(rows <= 65535, f"{rows} rows in one call; up to 65535")
+    num_pages, _, kv_heads, page_tokens, head_dim = pool.shape
+    _need(head_dim <= 512, f"head_dim {head_dim} is beyond 512")
+    _on_current_device(pool=pool.codes, out=out, block_tables=block_tables, row_request=row_request, first=first, last=last)
+    if rows and pool.codes.numel():
+        _call("mxb_read_cache", pool.codes.data_ptr(), pool.scales.data_ptr(), pool.kind, out.data_ptr(), _CODES[out.dtype],
+              block_tables.data_ptr(), block_tables.shape[1], row_request.data_ptr(), first.data_ptr(), last.data_ptr(), rows,
+              kv_heads, head_dim, page_tokens, num_pages, int(window or 0), int(chunk or 0), _kept(keep),
+              status_word(out.device).data_ptr(), _stream())
+    return out
+
+
 # ------------------------------------------------- q/k norm, rotation, cache
 def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out: Optional[torch.Tensor],
-                       cache: Optional[torch.Tensor], slots: Optional[torch.Tensor],
+                       cache, slots: Optional[torch.Tensor],
                        positions: torch.Tensor, q_weight: Optional[torch.Tensor],
                        k_weight: Optional[torch.Tensor], cos: Optional[torch.Tensor],
                        sin: Optional[torch.Tensor], eps: float, interleaved: bool = False,
@@ -1304,7 +1394,8 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
     (i, i + rotary_dim / 2), or (2i, 2i + 1) when ``interleaved``), q written to ``q_out``
     [tokens, heads, head_dim], k and v written into ``cache``
     [pages, 2, kv_heads, page_tokens, head_dim] at ``slots`` (a negative slot
-    skips the token; ``cache=None`` writes nothing). q, k and v are
+    skips the token; ``cache=None`` writes nothing; a ``QuantizedPool`` takes
+    the rows, unrounded, as codes and scales). q, k and v are
     [tokens, heads * head_dim] views whose rows may be strided. ``q_factors``
     (float32, one per position): what the queries are multiplied by."""
     dtype = q.dtype
@@ -1314,8 +1405,10 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
     tokens = q.shape[0]
     _check(positions, "positions", (torch.int32,), 1)
     _need(positions.numel() == tokens and k.shape[0] == tokens and v.shape[0] == tokens, "token counts differ")
+    quantized = isinstance(cache, QuantizedPool)
     if cache is not None:
-        _check(cache, "cache", (dtype,), 5)
+        if not quantized:
+            _check(cache, "cache", (dtype,), 5)
         num_pages, two, kv_heads, page_tokens, head_dim = cache.shape
         _need(two == 2, "cache must be [pages, 2, kv_heads, page_tokens, head_dim]")
         _check(slots, "slots", (torch.int32,), 1)
@@ -1348,6 +1441,19 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
         _need(rotary_dim <= head_dim, "rotary_dim exceeds head_dim")
     if q_factors is not None:
         _check(q_factors, "q_factors", (torch.float32,), 1)
+    if quantized:
+        _need(head_dim <= 512 and heads + 2 * kv_heads <= 65535, f"{heads} + 2 x {kv_heads} heads of {head_dim} values")
+        _on_current_device(cache=cache.codes, q=q, k=k, v=v, q_out=q_out, slots=slots, positions=positions, q_weight=q_weight,
+                           k_weight=k_weight, cos=cos, sin=sin, q_factors=q_factors)
+        projection = norm_scope == "projection" and (q_weight is not None or k_weight is not None)
+        sums = torch.empty(2 * tokens, dtype=torch.float32, device=q.device) if projection else None
+        _call("mxb_store_quantized", q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
+              _ptr(q_out), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.kind, slots.data_ptr(), positions.data_ptr(),
+              _ptr(q_weight), _ptr(k_weight), _ptr(cos), _ptr(sin), table_positions, rotary_dim, 1 if interleaved else 0,
+              1 if projection else 0, _ptr(sums), tokens, heads, kv_heads, head_dim, page_tokens, num_pages, float(eps),
+              _CODES[dtype], _ptr(q_factors), q_factors.numel() if q_factors is not None else 0,
+              status_word(q.device).data_ptr(), _stream())
+        return
     _call("mxb_qk_norm_rope_cache", q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0),
           v.stride(0), _ptr(q_out), _ptr(cache), _ptr(slots), positions.data_ptr(), _ptr(q_weight),
           _ptr(k_weight), _ptr(cos), _ptr(sin), table_positions, rotary_dim, 1 if interleaved else 0,
@@ -1371,9 +1477,10 @@ def norm_rotate_heads(x: torch.Tensor, head_dim: int, positions: torch.Tensor,
     return out
 
 
-def write_cache(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor,
+def write_cache(k: torch.Tensor, v: torch.Tensor, cache, slots: torch.Tensor,
                 positions: torch.Tensor) -> None:
-    """Stores k and v [tokens, kv_heads * head_dim] as they are at ``slots``."""
+    """Stores k and v [tokens, kv_heads * head_dim] as they are at ``slots``
+    (in a ``QuantizedPool``: as codes and scales)."""
     qk_norm_rope_cache(k[:, :0], k, v, None, cache, slots, positions, None, None, None, None, 0.0)
 
 
@@ -1604,7 +1711,53 @@ def set_decode_resident_blocks(blocks: int, many: int = 2048) -> None:
           "the number of resident blocks cannot be negative nor exceed that of a step with many pairs")
 
 
-def paged_attention_decode(q: torch.Tensor, cache: torch.Tensor, out: torch.Tensor,
+def quantized_decode_supported(head_dim: int, heads: int, kv_heads: int, dtype: torch.dtype) -> bool:
+    """Whether the decode attention takes this head layout over a ``QuantizedPool``."""
+    if dtype not in _CODES:
+        return False
+    return bool(_fn("mxb_paged_attention_decode_quantized_supported")(head_dim, heads, kv_heads, _CODES[dtype]))
+
+
+def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.Tensor], block_tables: torch.Tensor,
+                      row_token: torch.Tensor, row_request: torch.Tensor, positions: torch.Tensor, scale: float,
+                      longest_context: int, window: int, partial: Optional[torch.Tensor], chunk: int,
+                      gate: Optional[torch.Tensor], softcap: float, sink, bias, keep: int, weight: Optional[torch.Tensor],
+                      summands: Optional[torch.Tensor]) -> None:
+    """The decode attention over a quantized pool, into ``out`` or, with the
+    output projection ``weight``, into ``summands``."""
+    _need(softcap >= 0.0, "the cap on the scores cannot be negative")
+    tokens, heads, head_dim = q.shape
+    num_pages, _, kv_heads, page_tokens, cache_dim = pool.shape
+    _need(cache_dim == head_dim, f"the pool's rows are {cache_dim} values wide, the queries {head_dim}")
+    _need(quantized_decode_supported(head_dim, heads, kv_heads, q.dtype),
+          f"the decode attention over 8-bit rows does not take head_dim {head_dim} with {heads}/{kv_heads} heads in {q.dtype}")
+    _check(block_tables, "block_tables", (torch.int32,), 2)
+    for name, tensor in (("row_token", row_token), ("row_request", row_request), ("positions", positions)):
+        _check(tensor, name, (torch.int32,), 1)
+    rows = row_token.numel()
+    _need(row_request.numel() == rows and positions.numel() == tokens, "row lists do not fit")
+    _need(rows <= 65535, f"{rows} rows in one call; up to 65535")
+    splits = max(1, -(-int(longest_context) // decode_split_keys()))
+    need = rows * heads * splits * (head_dim + 2)
+    if partial is None:
+        partial = torch.empty(need, dtype=torch.float32, device=q.device)
+    _check(partial, "partial", (torch.float32,))
+    _need(partial.numel() >= need, f"partial holds {partial.numel()} values, {need} are needed")
+    gate_stride = _gate_stride(gate, q)
+    _on_current_device(cache=pool.codes, q=q, out=out, block_tables=block_tables, row_token=row_token, row_request=row_request,
+                       positions=positions, partial=partial, gate=gate, weight=weight)
+    hidden, ldw = (weight.shape[0], weight.stride(0)) if weight is not None else (0, 0)
+    if not rows:
+        return
+    _call("mxb_paged_attention_decode_quantized", q.data_ptr(), pool.codes.data_ptr(), pool.scales.data_ptr(), pool.kind,
+          _ptr(out), partial.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], row_token.data_ptr(),
+          row_request.data_ptr(), positions.data_ptr(), rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits,
+          int(window or 0), int(chunk or 0), _kept(keep), float(scale), _CODES[q.dtype], _ptr(weight), ldw, hidden,
+          _ptr(summands), _ptr(gate), gate_stride, float(softcap), *_sink(sink, heads), *_score_bias(bias, heads),
+          status_word(q.device).data_ptr(), _stream())
+
+
+def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
                            block_tables: torch.Tensor, row_token: torch.Tensor,
                            row_request: torch.Tensor, positions: torch.Tensor, scale: float,
                            longest_context: int, window: int = 0,
@@ -1623,13 +1776,19 @@ def paged_attention_decode(q: torch.Tensor, cache: torch.Tensor, out: torch.Tens
     more key that has no value and that every query sees (it joins the
     denominator where the splits are put together). ``bias`` (float32
     ``[heads, far + 1]``): joins the scores by head and distance. ``keep``: the
-    first that many positions are seen beside the window or chunk."""
+    first that many positions are seen beside the window or chunk. ``cache`` may
+    be a ``QuantizedPool``, with heads of any size up to 256 and any number of
+    query heads a key/value head."""
     dtype = q.dtype
     _need(softcap >= 0.0, "the cap on the scores cannot be negative")
     _check(q, "q", tuple(_CODES), 3)
     _check(out, "out", (dtype,), 3)
-    _check(cache, "cache", (dtype,), 5)
     _need(out.shape == q.shape, "out and q differ in shape")
+    if isinstance(cache, QuantizedPool):
+        _decode_quantized(q, cache, out, block_tables, row_token, row_request, positions, scale, longest_context, window,
+                          partial, chunk, gate, softcap, sink, bias, keep, None, None)
+        return out
+    _check(cache, "cache", (dtype,), 5)
     tokens, heads, head_dim = q.shape
     num_pages, two, kv_heads, page_tokens, cache_dim = cache.shape
     _need(two == 2 and cache_dim == head_dim, "cache must be [pages, 2, kv_heads, page_tokens, head_dim]")
@@ -1675,7 +1834,7 @@ def decode_project_supported(head_dim: int, heads: int, kv_heads: int, dtype: to
         head_dim, heads, kv_heads, _CODES[dtype], tokens, weight.data_ptr(), weight.stride(0)))
 
 
-def paged_attention_decode_project(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor,
+def paged_attention_decode_project(q: torch.Tensor, cache, block_tables: torch.Tensor,
                                    row_token: torch.Tensor, row_request: torch.Tensor, positions: torch.Tensor,
                                    scale: float, longest_context: int, weight: torch.Tensor,
                                    window: int = 0, chunk: int = 0,
@@ -1685,15 +1844,24 @@ def paged_attention_decode_project(q: torch.Tensor, cache: torch.Tensor, block_t
     ``weight`` ``[hidden, heads * head_dim]``, for steps of up to 64 tokens in
     bfloat16. Returns float32 ``[heads, tokens, hidden]``: the projection's sum
     over k left in one summand per head, for ``add_rmsnorm`` to add up. With
-    ``gate`` the heads' output is multiplied by sigmoid(gate) ahead of the projection."""
+    ``gate`` the heads' output is multiplied by sigmoid(gate) ahead of the projection.
+    ``cache`` may be a ``QuantizedPool``."""
     _check(q, "q", (torch.bfloat16,), 3)
-    _check(cache, "cache", (torch.bfloat16,), 5)
+    quantized = isinstance(cache, QuantizedPool)
+    if not quantized:
+        _check(cache, "cache", (torch.bfloat16,), 5)
     tokens, heads, head_dim = q.shape
     num_pages, two, kv_heads, page_tokens, cache_dim = cache.shape
     _need(two == 2 and cache_dim == head_dim, "cache must be [pages, 2, kv_heads, page_tokens, head_dim]")
     _need(weight.is_cuda and weight.dim() == 2 and weight.shape[1] == heads * head_dim, "weight does not fit the heads")
     _need(decode_project_supported(head_dim, heads, kv_heads, q.dtype, tokens, weight),
           f"the decode kernel with the projection does not take {tokens} tokens of {heads}/{kv_heads} heads of {head_dim}")
+    if quantized:
+        summands = torch.empty((heads, tokens, weight.shape[0]), dtype=torch.float32, device=q.device)
+        _need(row_token.numel() > 0, "no rows to project")
+        _decode_quantized(q, cache, None, block_tables, row_token, row_request, positions, scale, longest_context, window, None,
+                          chunk, gate, softcap, sink, bias, keep, weight, summands)
+        return summands
     _check(block_tables, "block_tables", (torch.int32,), 2)
     for name, tensor in (("row_token", row_token), ("row_request", row_request), ("positions", positions)):
         _check(tensor, name, (torch.int32,), 1)

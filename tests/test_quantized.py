@@ -1,0 +1,499 @@
+"""The cache held in 8 bits: rows written as codes and scales, pages read back, and the decode attention over the codes,
+each against its definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+LIMITS = {"fp8": 448.0, "int8": 127.0}
+F32, BF16 = torch.float32, torch.bfloat16
+HALF = {F32: 2.0 ** -24, BF16: 2.0 ** -8}    # a rounding's half step, relative to the value
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from metallix_b200 import ops
+    ops.require_cuda()
+    return ops
+
+
+def nearest_code(y, kind):
+    """The code nearest to y (float64), halves to the even one, as the number it stands for."""
+    if kind == "int8":
+        return y.round().clamp(-127, 127)
+    y = y.clamp(-448.0, 448.0)
+    step = torch.ldexp(torch.ones_like(y), torch.frexp(y).exponent.clamp(min=-5) - 4)
+    return (y / step).round() * step
+
+
+def exact_rows(x, kind):
+    """(scale, code values) of rows x [..., head_dim] of float32 or bfloat16 numbers, in 64 bits; the scale as float32 holds it."""
+    x = x.double()
+    scale = (x.abs().amax(-1).float() / torch.full((), LIMITS[kind], device=x.device)).double()
+    y = x / torch.where(scale > 0, scale, 1.0).unsqueeze(-1)
+    return scale, nearest_code(y, kind)
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def spread_tables(lengths, page, seed, spare=2):
+    """Block tables whose pages lie anywhere in the pool: (pages of the pool, tables [requests, width])."""
+    counts = [-(-n // page) for n in lengths]
+    gen = torch.Generator().manual_seed(seed)
+    order = torch.randperm(sum(counts) + spare, generator=gen).tolist()
+    table = torch.full((len(lengths), max(max(counts), 1)), -1, dtype=torch.int32)
+    for row, count in enumerate(counts):
+        for i in range(count):
+            table[row, i] = order.pop()
+    return sum(counts) + spare, table.cuda()
+
+
+def random_pool(ops, kind, pages, kv_heads, page, head_dim, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    pool = ops.QuantizedPool.zeros(pages, kv_heads, page, head_dim, codes=kind)
+    x = torch.randn(pool.shape, generator=gen, device="cuda")
+    scale, codes = exact_rows(x, kind)
+    pool.codes.copy_(codes.to(pool.codes.dtype))
+    pool.scales.copy_(scale)
+    return pool
+
+
+def values_of(pool):
+    """What the pool stands for, in float64."""
+    return pool.codes.float().double() * pool.scales.double().unsqueeze(-1)
+
+
+# ----------------------------------------------------------------- refusals, without a GPU
+def test_a_pool_says_what_is_wrong_with_it():
+    from metallix_b200 import ops
+    codes, scales = torch.zeros(3, 2, 1, 4, 8, dtype=torch.int8), torch.zeros(3, 2, 1, 4)
+    with pytest.raises(ops.KernelError, match="CUDA device"):
+        ops.QuantizedPool(codes, scales)
+    with pytest.raises(ops.KernelError, match="codes must be one of"):
+        ops.QuantizedPool.zeros(3, 1, 4, 8, codes="int4")
+    with pytest.raises(ops.KernelError, match="QuantizedPool"):
+        ops.read_cache(codes, codes, None, None, None, None)
+
+
+# ----------------------------------------------------------------- the write
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim,kv_heads,page,tokens", [(128, 2, 16, 37), (64, 5, 8, 33), (256, 1, 32, 9), (48, 3, 4, 21), (20, 2, 1, 6),
+                                                           (128, 8, 16, 1)])
+def test_rows_written_are_the_nearest_codes(ops, kind, dtype, head_dim, kv_heads, page, tokens):
+    """Keys and values as they are: scales and codes have one right answer each, bit for bit."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    wide = torch.randn((tokens, 3 * kv_heads * head_dim + 16), generator=gen, device="cuda").to(dtype)
+    k = wide[:, 8:8 + kv_heads * head_dim]               # rows of a wider product
+    v = wide[:, 8 + kv_heads * head_dim:8 + 2 * kv_heads * head_dim]
+    pages = -(-tokens // page) + 2
+    pool = random_pool(ops, kind, pages, kv_heads, page, head_dim, 3)
+    before_codes, before_scales = pool.codes.clone(), pool.scales.clone()
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(1))[:tokens].to(torch.int32)
+    if tokens > 5:
+        slots[4] = -1      # a token that is not written
+    ops.write_cache(k, v, pool, slots.cuda(), ints([0] * tokens))
+    ops.check_status("cuda")
+    written = slots.tolist()
+    for plane, rows in enumerate((k, v)):
+        scale, codes = exact_rows(rows.reshape(tokens, kv_heads, head_dim), kind)
+        for t, slot in enumerate(written):
+            if slot < 0:
+                continue
+            at = (slot // page, plane, slice(None), slot % page)
+            assert torch.equal(pool.scales[at].double(), scale[t])
+            assert torch.equal(pool.codes[at].float().double(), codes[t])
+            before_codes[at], before_scales[at] = pool.codes[at], pool.scales[at]
+    # everything else is as it was
+    assert torch.equal(pool.codes.view(torch.uint8), before_codes.view(torch.uint8)) and torch.equal(pool.scales, before_scales)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("head_dim", [128, 48])
+def test_quotients_next_to_the_middle_of_two_codes(ops, kind, head_dim):
+    """Numbers an ulp to either side of, and on, the middle between two codes, at scales from 2^-140 to 2^118."""
+    gen = torch.Generator().manual_seed(7)
+    rows = []
+    for exponent in (-140, -127, -100, -61, -60, -3, 0, 5, 59, 61, 100, 118):
+        for mantissa in (1.0, 1.0 + 2.0 ** -23, 1.37, 2.0 - 2.0 ** -23):
+            top = torch.tensor(mantissa * 2.0 ** exponent, dtype=F32)
+            scale = top / LIMITS[kind]
+            values = torch.arange(-126, 127).double() + 0.5 if kind == "int8" else \
+                torch.tensor([(8 + i + 0.5) * 2.0 ** (e - 3) for i in range(8) for e in range(-6, 8)] + [(i + 0.5) * 2.0 ** -9 for i in range(8)]).double()
+            middle = values[torch.randint(len(values), (head_dim - 1,), generator=gen)] * scale.double()
+            x = middle.float()
+            step = torch.randint(-1, 2, (head_dim - 1,), generator=gen)
+            x = torch.where(step > 0, torch.nextafter(x, torch.tensor(math.inf)), torch.where(step < 0, torch.nextafter(x, torch.tensor(-math.inf)), x))
+            rows.append(torch.cat([top.reshape(1), x.clamp(-top, top)]))
+    k = torch.stack(rows).cuda()
+    tokens = k.shape[0]
+    pool = ops.QuantizedPool.zeros(tokens, 1, 1, head_dim, codes=kind)
+    ops.write_cache(k, -k, pool, ints(list(range(tokens))), ints([0] * tokens))
+    for plane, x in enumerate((k, -k)):
+        scale, codes = exact_rows(x, kind)
+        assert torch.equal(pool.scales[:, plane, 0, 0].double(), scale)
+        assert torch.equal(pool.codes[:, plane, 0, 0].float().double(), codes)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("head_dim", [64, 20])
+def test_rows_of_zeros_and_rows_that_are_not_finite(ops, kind, head_dim):
+    k = torch.ones(5, head_dim, device="cuda")
+    k[0] = 0.0
+    k[1, 3] = math.inf
+    k[2, head_dim - 1] = math.nan
+    k[3, 0] = -math.inf
+    k[4] = 1e-45          # the smallest number there is
+    pool = ops.QuantizedPool.zeros(5, 1, 1, head_dim, codes=kind)
+    pool.codes.view(torch.uint8).fill_(0x11)
+    ops.write_cache(k, k, pool, ints(range(5)), ints([0] * 5))
+    assert pool.scales[0].eq(0).all() and pool.scales[1:4].isnan().all()
+    out = torch.full(pool.shape, 7.0, device="cuda")
+    ops.read_cache(pool, out, ints([[0], [1], [2], [3], [4]]), ints(range(5)), ints([0] * 5), ints([0] * 5))
+    assert out[0].eq(0).all() and out[1:4].isnan().all() and out[4].isfinite().all()
+    ops.check_status("cuda")
+
+
+def turned(x, cos, sin, positions, interleaved):
+    """Rotation of [tokens, heads, head_dim] in float64."""
+    half = cos.shape[1]
+    where = torch.arange(half, device=x.device)
+    i, j = (2 * where, 2 * where + 1) if interleaved else (where, where + half)
+    c, s = cos.double()[positions.long()].unsqueeze(1), sin.double()[positions.long()].unsqueeze(1)
+    out = x.clone()
+    out[..., i] = x[..., i] * c - x[..., j] * s
+    out[..., j] = x[..., j] * c + x[..., i] * s
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim,heads,kv_heads,rotary,interleaved,scope,tokens", [
+    (128, 4, 2, 128, False, "head", 19), (64, 6, 2, 64, True, "head", 7), (128, 8, 4, 64, False, "head", 40),
+    (256, 2, 1, 256, False, "head", 5), (48, 3, 1, 24, False, "head", 11), (128, 4, 2, 128, False, "projection", 6),
+    (20, 4, 2, 12, True, "projection", 5), (64, 4, 4, 0, False, "head", 9), (128, 16, 8, 128, False, None, 3),
+    (256, 4, 4, 64, True, None, 13), (128, 32, 8, 128, False, "head", 700), (64, 15, 5, 64, True, None, 900)])
+def test_norm_rotation_and_write(ops, kind, dtype, head_dim, heads, kv_heads, rotary, interleaved, scope, tokens):
+    """Queries as the write into a cache of the compute type gives them; keys: a code is the nearest one to the quotient, but
+    for what the row's own rounding in 32 bits moves it by."""
+    gen = torch.Generator(device="cuda").manual_seed(head_dim + tokens)
+    width = (heads + 2 * kv_heads) * head_dim
+    qkv = torch.randn((tokens, width), generator=gen, device="cuda").to(dtype)
+    q, k, v = qkv.split([heads * head_dim, kv_heads * head_dim, kv_heads * head_dim], 1)
+    positions = torch.randint(0, 300, (tokens,), generator=gen, device="cuda").to(torch.int32)
+    page, pages = 8, -(-tokens // 8) + 1
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(5))[:tokens].to(torch.int32).cuda()
+    weight = lambda n: 1.0 + 0.2 * torch.randn(n, generator=gen, device="cuda")  # noqa: E731
+    whole = scope == "projection"
+    qw, kw = (weight(heads * head_dim if whole else head_dim), weight(kv_heads * head_dim if whole else head_dim)) if scope else (None, None)
+    cos = sin = None
+    if rotary:
+        angle = torch.rand((300, rotary // 2), generator=gen, device="cuda") * 6.28
+        cos, sin = angle.cos(), angle.sin()
+    factors = 0.5 + torch.rand(300, generator=gen, device="cuda")
+    pool = ops.QuantizedPool.zeros(pages, kv_heads, page, head_dim, codes=kind)
+    plain = torch.zeros(pool.shape, dtype=dtype, device="cuda")
+    outs = [torch.zeros((tokens, heads, head_dim), dtype=dtype, device="cuda") for _ in range(2)]
+    for cache, out in zip((pool, plain), outs):
+        ops.qk_norm_rope_cache(q, k, v, out, cache, slots, positions, qw, kw, cos, sin, 1e-6, interleaved=interleaved,
+                               norm_scope=scope or "head", q_factors=factors)
+    ops.check_status("cuda")
+
+    def exact(x, w):
+        x = x.double().reshape(tokens, -1, head_dim)
+        if w is not None:
+            mean = x.square().mean((1, 2), keepdim=True) if whole else x.square().mean(-1, keepdim=True)
+            x = x * torch.rsqrt(mean + 1e-6) * (w.double().view(-1, head_dim) if whole else w.double())
+        return turned(x, cos, sin, positions, interleaved) if rotary else x
+
+    # a value in 32 bits: the row's sum of squares and root, two products, and a rotation of two more products and a sum
+    bits = 16 * 2.0 ** -24
+    query = exact(q, qw) * factors.double()[positions.long()][:, None, None]
+    size = query.abs().amax(-1, keepdim=True)
+    for out in outs:
+        assert ((out.double() - query).abs() <= HALF[dtype] * query.abs() + bits * 1.5 * size).all()
+    held, row = slots.long() // page, slots.long() % page
+    key = exact(k, kw)
+    scale = pool.scales[held, 0, :, row].double()
+    size = key.abs().amax(-1)
+    assert ((scale * LIMITS[kind] - size).abs() <= 2 * bits * size).all()
+    code = pool.codes[held, 0, :, row].float().double()
+    y = key / scale.unsqueeze(-1)
+    off = (code - y).abs()
+    best = (nearest_code(y, kind) - y).abs()
+    assert (off <= best + 2 * 2 * bits * LIMITS[kind]).all()      # another code only where both are as near
+    value_scale, value_codes = exact_rows(v.reshape(tokens, kv_heads, head_dim), kind)
+    assert torch.equal(pool.scales[held, 1, :, row].double(), value_scale)
+    assert torch.equal(pool.codes[held, 1, :, row].float().double(), value_codes)
+
+
+@gpu
+def test_a_slot_or_position_outside_its_table_is_reported(ops):
+    pool = ops.QuantizedPool.zeros(2, 1, 4, 64)
+    k = torch.ones(2, 64, device="cuda", dtype=BF16)
+    ops.write_cache(k, k, pool, ints([8, 0]), ints([0, 0]))
+    with pytest.raises(ops.KernelError, match="slot or position"):
+        ops.check_status("cuda")
+    assert pool.scales[0, 0, 0, 0] > 0 and pool.scales.count_nonzero() == 2
+    cos = torch.ones(4, 32, device="cuda")
+    ops.qk_norm_rope_cache(k[:, :0], k, k, None, pool, ints([1, 2]), ints([4, -1]), None, None, cos, cos, 0.0)
+    with pytest.raises(ops.KernelError, match="slot or position"):
+        ops.check_status("cuda")
+
+
+@gpu
+def test_refusals_of_the_write(ops):
+    pool = ops.QuantizedPool.zeros(2, 1, 4, 64)
+    k = torch.ones(2, 64, device="cuda", dtype=BF16)
+    with pytest.raises(ops.KernelError, match="widths"):
+        ops.write_cache(k[:, :32], k[:, :32], pool, ints([0, 1]), ints([0, 0]))
+    with pytest.raises(ops.KernelError, match="one slot per token"):
+        ops.write_cache(k, k, pool, ints([0]), ints([0, 0]))
+    with pytest.raises(ops.KernelError, match="one scale per row"):
+        ops.QuantizedPool(pool.codes, pool.scales[:, :1].contiguous())
+    with pytest.raises(ops.KernelError, match="dtype"):
+        ops.QuantizedPool(pool.codes.view(torch.uint8), pool.scales)
+    with pytest.raises(ops.KernelError, match="contiguous"):
+        ops.QuantizedPool(pool.codes.transpose(3, 4), pool.scales)
+
+
+# ----------------------------------------------------------------- reading back
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim,kv_heads,page", [(128, 2, 16), (64, 3, 8), (256, 1, 64), (40, 2, 4), (24, 1, 1), (13, 2, 2)])
+@pytest.mark.parametrize("window,chunk,keep", [(0, 0, 0), (9, 0, 0), (0, 32, 0), (20, 0, 6)])
+def test_pages_read_back(ops, kind, dtype, head_dim, kv_heads, page, window, chunk, keep):
+    lengths = [1, 50, 0, 77, 16, 33]
+    firsts = [0, 45, 0, 40, 15, 0]
+    pages, table = spread_tables(lengths, page, 2)
+    pool = random_pool(ops, kind, pages, kv_heads, page, head_dim, 4)
+    order = [3, 0, 5, 1, 4, 2]
+    out = torch.full(pool.shape, 7.0, dtype=dtype, device="cuda")
+    ops.read_cache(pool, out, table, ints(order), ints([firsts[r] for r in order]), ints([lengths[r] - 1 for r in order]),
+                   window=window, chunk=chunk, keep=keep)
+    ops.check_status("cuda")
+    expect = torch.full(pool.shape, 7.0, dtype=dtype, device="cuda")
+    values = (pool.codes.float() * pool.scales.unsqueeze(-1)).to(dtype)
+    for r, length in enumerate(lengths):
+        begin = max(firsts[r] - window + 1, 0) if window else 0
+        if chunk:
+            begin = max(begin, firsts[r] - firsts[r] % chunk)
+        for slot in range(-(-length // page)):
+            if (slot + 1) * page <= begin and slot * page >= keep:
+                continue
+            at, rows = int(table[r, slot]), min(page, length - slot * page)
+            expect[at, :, :, :rows] = values[at, :, :, :rows]
+    assert torch.equal(out, expect)
+
+
+@gpu
+def test_a_page_outside_the_pool_is_reported_and_not_read(ops):
+    pool = random_pool(ops, "fp8", 3, 1, 4, 64, 0)
+    out = torch.zeros(pool.shape, device="cuda")
+    ops.read_cache(pool, out, ints([[1, 3, -1]]), ints([0]), ints([0]), ints([11]))
+    with pytest.raises(ops.KernelError, match="block-table"):
+        ops.check_status("cuda")
+    assert out[1].abs().sum() > 0 and out[0].eq(0).all() and out[2].eq(0).all()
+    with pytest.raises(ops.KernelError, match="pool's shape"):
+        ops.read_cache(pool, out[:2], ints([[1]]), ints([0]), ints([0]), ints([3]))
+    with pytest.raises(ops.KernelError, match="differ in length"):
+        ops.read_cache(pool, out, ints([[1]]), ints([0]), ints([0, 0]), ints([3]))
+
+
+# ----------------------------------------------------------------- the decode attention
+def exact_decode(q, pool, table, rows, positions, scale, window=0, chunk=0, keep=0, softcap=0.0, sink=None, bias=None, gate=None):
+    """(out, bound) [tokens, heads, head_dim] in float64 of the rows (token, request): what comes out, and the sum of the
+    weights times the values' magnitudes, which roundings of the weights are relative to."""
+    values = values_of(pool)
+    page, kv_heads = pool.shape[3], pool.shape[2]
+    tokens, heads, head_dim = q.shape
+    out, bound = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))
+    for token, request in rows:
+        pos = int(positions[token])
+        at = torch.arange(pos + 1)
+        first = max(pos - window + 1, 0) if window else 0
+        if chunk:
+            first = max(first, pos - pos % chunk)
+        at = at[(at >= first) | (at < keep)]
+        held, row = table[request].cpu().long()[at // page].cuda(), (at % page).cuda()
+        keys, vals = (values[held, plane, :, row].repeat_interleave(heads // kv_heads, 1) for plane in (0, 1))
+        s = torch.einsum("hd,khd->hk", q[token].double(), keys) * scale
+        if softcap:
+            s = softcap * torch.tanh(s / softcap)
+        if bias is not None:
+            s = s + bias.double()[:, (pos - at).clamp(max=bias.shape[1] - 1).cuda()]
+        if sink is not None:
+            extra = sink.double() if isinstance(sink, torch.Tensor) else torch.full((heads,), sink, dtype=torch.float64, device="cuda")
+            s = torch.cat([s, extra[:, None]], 1)
+        p = torch.softmax(s, 1)[:, :len(at)]
+        out[token] = torch.einsum("hk,khd->hd", p, vals)
+        bound[token] = torch.einsum("hk,khd->hd", p, vals.abs())
+        if gate is not None:
+            g = torch.sigmoid(gate[token].double().view(heads, head_dim))
+            out[token] *= g
+            bound[token] *= g
+    return out, bound
+
+
+def close(out, exact, bound, dtype):
+    """Weights in bfloat16 (in its type alone), the output's own rounding, and what a score's rounding in 32 bits does to
+    its exponential: scores of up to some 30, sums of up to 256 products, 2^-24 each, three roundings of the sums."""
+    per_weight = (HALF[BF16] if dtype == BF16 else 0.0) + 30 * 8 * 2.0 ** -24
+    off = (out.double() - exact).abs()
+    limit = per_weight * bound + HALF[dtype] * exact.abs() * 1.01 + 1e-30
+    assert (off <= limit).all(), f"{(off / limit).max().item():.2f} times the bound"
+
+
+SHAPES = [(128, 2, 2, 16), (128, 8, 1, 16), (64, 14, 2, 32), (128, 15, 3, 8), (256, 4, 2, 16), (64, 4, 4, 4), (64, 3, 3, 1), (128, 6, 1, 256),
+          (48, 6, 2, 16), (20, 3, 1, 8), (128, 24, 2, 64), (256, 8, 1, 2)]
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim,heads,kv_heads,page", SHAPES)
+@pytest.mark.parametrize("lengths", [[1], [2, 129, 128, 127], [700, 1, 33, 2500], [5000, 4097]])
+def test_decode(ops, kind, dtype, head_dim, heads, kv_heads, page, lengths):
+    pages, table = spread_tables(lengths, page, 1)
+    pool = random_pool(ops, kind, pages, kv_heads, page, head_dim, 2)
+    # what lies behind a request's last position, and on pages that nobody holds, is no number
+    for r, n in enumerate(lengths):
+        if n % page:
+            pool.scales[int(table[r, n // page]), :, :, n % page:] = math.nan
+    held = set(table[table >= 0].flatten().tolist())
+    for free in set(range(pages)) - held:
+        pool.scales[free] = math.inf
+        pool.codes.view(torch.uint8)[free] = 0x7f
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    n = len(lengths)
+    q = torch.randn((n + 2, heads, head_dim), generator=gen, device="cuda").to(dtype)
+    positions = torch.zeros(n + 2, dtype=torch.int32, device="cuda")
+    tokens = [(3 * r + 1) % (n + 2) if math.gcd(3, n + 2) == 1 else r for r in range(n)]
+    rows = list(zip(tokens, range(n)))
+    for token, r in rows:
+        positions[token] = lengths[r] - 1
+    out = torch.full(q.shape, 5.0, dtype=dtype, device="cuda")
+    scale = 1.0 / math.sqrt(head_dim)
+    got = ops.paged_attention_decode(q, pool, out, table, ints([rows[0][0], -1] + [t for t, _ in rows[1:]]),
+                                     ints([0, 0] + list(range(1, n))), positions, scale, max(lengths))
+    ops.check_status("cuda")
+    assert got is out
+    exact, bound = exact_decode(q, pool, table, rows, positions, scale)
+    close(out[tokens], exact[tokens], bound[tokens], dtype)
+    others = [t for t in range(n + 2) if t not in tokens]
+    assert out[others].eq(5.0).all()      # tokens that no row names
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim,heads,kv_heads,page", [(128, 8, 2, 16), (64, 7, 1, 8), (256, 4, 2, 32), (40, 4, 2, 4)])
+@pytest.mark.parametrize("options", [dict(window=1), dict(window=300), dict(chunk=256), dict(window=100, keep=5), dict(window=130, keep=200),
+                                     dict(softcap=3.0), dict(sink=0.5), dict(sink="heads"), dict(bias=64), dict(gate=True),
+                                     dict(window=64, softcap=5.0, sink="heads", bias=3, gate=True, keep=1)],
+                         ids=lambda o: "-".join(f"{k}{v}" for k, v in o.items()))
+def test_decode_options(ops, dtype, head_dim, heads, kv_heads, page, options):
+    lengths = [900, 3, 257, 1500, 128]
+    pages, table = spread_tables(lengths, page, 3)
+    pool = random_pool(ops, "fp8", pages, kv_heads, page, head_dim, 6)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    n = len(lengths)
+    q = torch.randn((n, heads, head_dim), generator=gen, device="cuda").to(dtype)
+    positions = ints([x - 1 for x in lengths])
+    options = dict(options)
+    if options.get("sink") == "heads":
+        options["sink"] = torch.randn(heads, generator=gen, device="cuda")
+    if "bias" in options:
+        options["bias"] = torch.randn((heads, options["bias"] + 1), generator=gen, device="cuda")
+    if options.get("gate"):
+        options["gate"] = torch.randn((n, 2 * heads * head_dim), generator=gen, device="cuda").to(dtype)[:, :heads * head_dim]
+    if options.get("window"):      # pages ahead of the window have left the table, but for those that are kept
+        for r, length in enumerate(lengths):
+            for slot in range(max(length - options["window"], 0) // page):
+                if slot * page >= options.get("keep", 0):
+                    table[r, slot] = -1
+    out = torch.zeros_like(q)
+    scale = 1.0 / math.sqrt(head_dim)
+    ops.paged_attention_decode(q, pool, out, table, ints(range(n)), ints(range(n)), positions, scale, 1500, **options)
+    ops.check_status("cuda")
+    exact, bound = exact_decode(q, pool, table, [(r, r) for r in range(n)], positions, scale, **options)
+    if options.get("gate") is not None:      # the gate's own exponential and product
+        bound = bound * (1 + 1e-4)
+    close(out, exact, bound, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("head_dim,heads,kv_heads", [(128, 8, 2), (64, 7, 1)])
+def test_decode_with_the_output_projection(ops, kind, head_dim, heads, kv_heads):
+    lengths, hidden = [900, 3, 257], 200
+    pages, table = spread_tables(lengths, 16, 3)
+    pool = random_pool(ops, kind, pages, kv_heads, 16, head_dim, 6)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn((4, heads, head_dim), generator=gen, device="cuda").to(BF16)
+    w = (0.05 * torch.randn((hidden, heads * head_dim), generator=gen, device="cuda")).to(BF16)
+    positions, scale = ints([899, 2, 256, 0]), 1.0 / math.sqrt(head_dim)
+    arguments = (table, ints([0, 1, 2, -1]), ints([0, 1, 2, 0]), positions, scale, 900)
+    out = torch.zeros_like(q)
+    ops.paged_attention_decode(q, pool, out, *arguments)
+    summands = ops.paged_attention_decode_project(q, pool, *arguments, w)
+    ops.check_status("cuda")
+    assert summands.shape == (heads, 4, hidden) and summands[:, 3].eq(0).all()
+    parts = torch.einsum("thd,nhd->htn", out.double(), w.double().view(hidden, heads, head_dim))
+    size = torch.einsum("thd,nhd->htn", out.double().abs(), w.double().abs().view(hidden, heads, head_dim))
+    assert ((summands.double() - parts).abs() <= head_dim * 2.0 ** -24 * 4 * size + 1e-30).all()
+
+
+@gpu
+def test_decode_of_rows_that_are_not_finite_shows_it(ops):
+    pool = random_pool(ops, "fp8", 2, 2, 16, 128, 0)
+    pool.scales[0, 1, 1, 3] = math.nan      # a value of the second key/value head
+    q = torch.ones(1, 4, 128, device="cuda", dtype=BF16)
+    out = torch.zeros_like(q)
+    ops.paged_attention_decode(q, pool, out, ints([[0, 1]]), ints([0]), ints([0]), ints([19]), 0.1, 20)
+    assert out[0, 2:].isnan().all() and out[0, :2].isfinite().all()
+
+
+@gpu
+def test_decode_reports_pages_and_contexts_beyond_their_bounds(ops):
+    pool = random_pool(ops, "int8", 2, 1, 16, 64, 0)
+    q = torch.ones(1, 2, 64, device="cuda", dtype=BF16)
+    out = torch.zeros_like(q)
+    for table in ([[0, 2]], [[0, -1]], [[0]]):
+        ops.paged_attention_decode(q, pool, out, ints(table), ints([0]), ints([0]), ints([19]), 0.1, 20)
+        with pytest.raises(ops.KernelError, match="block-table"):
+            ops.check_status("cuda")
+    big = random_pool(ops, "int8", 10, 1, 16, 64, 0)
+    out.fill_(3.0)
+    ops.paged_attention_decode(q, big, out, ints([list(range(10))]), ints([0]), ints([0]), ints([150]), 0.1, 128)
+    with pytest.raises(ops.KernelError, match="position"):
+        ops.check_status("cuda")
+    assert out.eq(3.0).all()
+
+
+@gpu
+def test_refusals_of_the_decode_attention(ops):
+    pool = random_pool(ops, "fp8", 2, 2, 16, 64, 0)
+    q = torch.ones(1, 4, 64, device="cuda", dtype=BF16)
+    lists = (ints([[0, 1]]), ints([0]), ints([0]), ints([3]), 0.1, 20)
+    with pytest.raises(ops.KernelError, match="64 values wide"):
+        ops.paged_attention_decode(q[..., :32].contiguous(), pool, q[..., :32].contiguous(), *lists)
+    with pytest.raises(ops.KernelError, match="does not take"):
+        ops.paged_attention_decode(q[:, :3].contiguous(), pool, torch.zeros_like(q[:, :3]), *lists)
+    with pytest.raises(ops.KernelError, match="negative"):
+        ops.paged_attention_decode(q, pool, torch.zeros_like(q), *lists, softcap=-1.0)
+    with pytest.raises(ops.KernelError, match="partial holds"):
+        ops.paged_attention_decode(q, pool, torch.zeros_like(q), *lists, partial=torch.zeros(8, device="cuda"))
+    with pytest.raises(ops.KernelError, match="row lists"):
+        ops.paged_attention_decode(q, pool, torch.zeros_like(q), ints([[0, 1]]), ints([0]), ints([0, 0]), ints([3]), 0.1, 20)
+    for other in (ops.paged_attention_tile, ops.flash_prefill):      # the kernels that read a cache of the compute type say so
+        with pytest.raises(ops.KernelError, match="cache must be a tensor"):
+            other(q, pool, torch.zeros_like(q), ints([[0, 1]]), ints([0]), ints([0]), ints([1]), ints([3]), 0.1)
