@@ -1303,14 +1303,16 @@ MXB_API int mxb_paged_attention_decode_quantized_supported(int head_dim, int hea
 // page_tokens, head_dim] and scales [pages, 2, kv_heads, page_tokens]. With w
 // (bfloat16 heads of 64 or 128 values, up to 64 tokens) the partial results are
 // put together and projected by one kernel, as mxb_paged_attention_decode_project does.
+// settled: with chained launches on, the positions ahead of each token's own were
+// written by launches before the last one, and may be fetched while that one runs.
 MXB_API int mxb_paged_attention_decode_quantized(const void* q, const void* codes, const float* scales, int kind, void* out, float* partial,
                                                  const int* block_tables, int max_pages, const int* row_token, const int* row_request,
                                                  const int* positions, int rows, int tokens, int heads, int kv_heads, int head_dim,
                                                  int page_tokens, int num_pages, int max_splits, int window, int chunk, int keep,
                                                  float scale, int dtype, const void* w, long long ldw, int hidden, float* summands,
                                                  const void* gate, long long gate_stride, float softcap, int has_sink, float sink_score,
-                                                 const float* sink_heads, const float* bias_table, int bias_far, int* status,
-                                                 cudaStream_t stream) {
+                                                 const float* sink_heads, const float* bias_table, int bias_far, int settled,
+                                                 int* status, cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (!mxb_paged_attention_decode_quantized_supported(head_dim, heads, kv_heads, dtype) || max_splits <= 0 || page_tokens <= 0 ||
       num_pages <= 0 || rows > 65535 || (kind != kCodesE4M3 && kind != kCodesInt8) || (bias_table != nullptr && bias_far < 0) ||
@@ -1320,10 +1322,10 @@ MXB_API int mxb_paged_attention_decode_quantized(const void* q, const void* code
     return static_cast<int>(cudaErrorInvalidValue);
   const QuantizedDecode args = {q, static_cast<const uint8_t*>(codes), scales, partial, block_tables, max_pages, row_token, row_request,
                                 positions, heads, kv_heads, head_dim, page_tokens, num_pages, window, chunk, keep, scale, softcap,
-                                ScoreBias{bias_table, bias_far}, status};
-  const int slots = quantized_slots(rows * kv_heads, max_splits);
-  const cudaError_t e = dtype == kF32 ? launch_quantized_decode<float>(args, kind, rows, slots, stream)
-                                      : launch_quantized_decode<__nv_bfloat16>(args, kind, rows, slots, stream);
+                                ScoreBias{bias_table, bias_far}, settled, status};
+  int slots = 1;
+  const cudaError_t e = dtype == kF32 ? launch_quantized_decode<float>(args, kind, rows, max_splits, &slots, stream)
+                                      : launch_quantized_decode<__nv_bfloat16>(args, kind, rows, max_splits, &slots, stream);
   if (e != cudaSuccess) return static_cast<int>(e);
   if (w != nullptr) {
     auto project = head_dim == 64 ? launch_merge_project<64> : launch_merge_project<128>;

@@ -92,7 +92,7 @@ _SIGNATURES = {
                                    _F, _I, _P, _L, _F, _I, _F, _P, _P, _I, _P, _P],
     "mxb_paged_attention_decode_quantized_supported": [_I, _I, _I, _I],
     "mxb_paged_attention_decode_quantized": [_P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
-                                             _F, _I, _P, _L, _I, _P, _P, _L, _F, _I, _F, _P, _P, _I, _P, _P],
+                                             _F, _I, _P, _L, _I, _P, _P, _L, _F, _I, _F, _P, _P, _I, _I, _P, _P],
     "mxb_store_quantized": [_P, _P, _P, _L, _L, _L, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _I, _I, _I, _I, _I,
                             _F, _I, _P, _I, _P, _P],
     "mxb_read_cache": [_P, _P, _I, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
@@ -1721,8 +1721,8 @@ def quantized_decode_supported(head_dim: int, heads: int, kv_heads: int, dtype: 
 def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.Tensor], block_tables: torch.Tensor,
                       row_token: torch.Tensor, row_request: torch.Tensor, positions: torch.Tensor, scale: float,
                       longest_context: int, window: int, partial: Optional[torch.Tensor], chunk: int,
-                      gate: Optional[torch.Tensor], softcap: float, sink, bias, keep: int, weight: Optional[torch.Tensor],
-                      summands: Optional[torch.Tensor]) -> None:
+                      gate: Optional[torch.Tensor], softcap: float, sink, bias, keep: int, settled: bool,
+                      weight: Optional[torch.Tensor], summands: Optional[torch.Tensor]) -> None:
     """The decode attention over a quantized pool, into ``out`` or, with the
     output projection ``weight``, into ``summands``."""
     _need(softcap >= 0.0, "the cap on the scores cannot be negative")
@@ -1754,7 +1754,7 @@ def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.
           row_request.data_ptr(), positions.data_ptr(), rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits,
           int(window or 0), int(chunk or 0), _kept(keep), float(scale), _CODES[q.dtype], _ptr(weight), ldw, hidden,
           _ptr(summands), _ptr(gate), gate_stride, float(softcap), *_sink(sink, heads), *_score_bias(bias, heads),
-          status_word(q.device).data_ptr(), _stream())
+          1 if settled else 0, status_word(q.device).data_ptr(), _stream())
 
 
 def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
@@ -1763,7 +1763,7 @@ def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
                            longest_context: int, window: int = 0,
                            partial: Optional[torch.Tensor] = None, chunk: int = 0,
                            gate: Optional[torch.Tensor] = None, softcap: float = 0.0,
-                           sink=None, bias=None, keep: int = 0) -> torch.Tensor:
+                           sink=None, bias=None, keep: int = 0, settled: bool = False) -> torch.Tensor:
     """Attention of single tokens over their requests' cached keys, split
     along the keys. ``row_token[i]`` is the token (row of q and out) of the
     i-th decoded request, negative for a padding row; ``row_request[i]`` its
@@ -1778,7 +1778,10 @@ def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
     ``[heads, far + 1]``): joins the scores by head and distance. ``keep``: the
     first that many positions are seen beside the window or chunk. ``cache`` may
     be a ``QuantizedPool``, with heads of any size up to 256 and any number of
-    query heads a key/value head."""
+    query heads a key/value head; then ``settled`` says that the positions ahead
+    of each token's own were written by launches before the last one, so that
+    with chained launches on they may be fetched while that one runs (a cache in
+    the compute type is taken to be so)."""
     dtype = q.dtype
     _need(softcap >= 0.0, "the cap on the scores cannot be negative")
     _check(q, "q", tuple(_CODES), 3)
@@ -1786,7 +1789,7 @@ def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
     _need(out.shape == q.shape, "out and q differ in shape")
     if isinstance(cache, QuantizedPool):
         _decode_quantized(q, cache, out, block_tables, row_token, row_request, positions, scale, longest_context, window,
-                          partial, chunk, gate, softcap, sink, bias, keep, None, None)
+                          partial, chunk, gate, softcap, sink, bias, keep, settled, None, None)
         return out
     _check(cache, "cache", (dtype,), 5)
     tokens, heads, head_dim = q.shape
@@ -1839,13 +1842,13 @@ def paged_attention_decode_project(q: torch.Tensor, cache, block_tables: torch.T
                                    scale: float, longest_context: int, weight: torch.Tensor,
                                    window: int = 0, chunk: int = 0,
                                    gate: Optional[torch.Tensor] = None, softcap: float = 0.0,
-                                   sink=None, bias=None, keep: int = 0) -> torch.Tensor:
+                                   sink=None, bias=None, keep: int = 0, settled: bool = False) -> torch.Tensor:
     """``paged_attention_decode`` followed at once by the output projection
     ``weight`` ``[hidden, heads * head_dim]``, for steps of up to 64 tokens in
     bfloat16. Returns float32 ``[heads, tokens, hidden]``: the projection's sum
     over k left in one summand per head, for ``add_rmsnorm`` to add up. With
     ``gate`` the heads' output is multiplied by sigmoid(gate) ahead of the projection.
-    ``cache`` may be a ``QuantizedPool``."""
+    ``cache`` may be a ``QuantizedPool``, with ``settled`` as there."""
     _check(q, "q", (torch.bfloat16,), 3)
     quantized = isinstance(cache, QuantizedPool)
     if not quantized:
@@ -1860,7 +1863,7 @@ def paged_attention_decode_project(q: torch.Tensor, cache, block_tables: torch.T
         summands = torch.empty((heads, tokens, weight.shape[0]), dtype=torch.float32, device=q.device)
         _need(row_token.numel() > 0, "no rows to project")
         _decode_quantized(q, cache, None, block_tables, row_token, row_request, positions, scale, longest_context, window, None,
-                          chunk, gate, softcap, sink, bias, keep, weight, summands)
+                          chunk, gate, softcap, sink, bias, keep, settled, weight, summands)
         return summands
     _check(block_tables, "block_tables", (torch.int32,), 2)
     for name, tensor in (("row_token", row_token), ("row_request", row_request), ("positions", positions)):
