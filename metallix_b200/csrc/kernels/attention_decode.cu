@@ -1295,9 +1295,28 @@ MXB_API int mxb_paged_attention_decode_project(const void* q, const void* cache,
 }
 
 // Whether the decode kernels over a cache in 8 bits take this head layout.
-MXB_API int mxb_paged_attention_decode_quantized_supported(int head_dim, int heads, int kv_heads, int dtype) {
-  return head_dim > 0 && head_dim <= 256 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && (dtype == kF32 || dtype == kBF16) ? 1 : 0;
+static bool quantized_decode_takes(int head_dim, int heads, int kv_heads, int dtype) {
+  return head_dim > 0 && head_dim <= 256 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && (dtype == kF32 || dtype == kBF16);
 }
+
+// What mxb_paged_attention_decode_quantized is asked for, 8 bytes a field (one
+// pointer crosses into the library instead of forty arguments, which a caller
+// in Python pays 4 us for).
+struct QuantizedDecodeCall {
+  const void *q, *codes;
+  const float* scales;
+  void* out;
+  float* partial;
+  const int *block_tables, *row_token, *row_request, *positions;
+  const void* w;
+  float* summands;
+  const void* gate;
+  const float *sink_heads, *bias_table;
+  int* status;
+  long long kind, dtype, max_pages, rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, max_splits, window, chunk, keep,
+      ldw, hidden, gate_stride, has_sink, bias_far, settled;
+  double scale, softcap, sink_score;
+};
 
 // mxb_paged_attention_decode over a cache in 8 bits: codes [pages, 2, kv_heads,
 // page_tokens, head_dim] and scales [pages, 2, kv_heads, page_tokens]. With w
@@ -1305,45 +1324,48 @@ MXB_API int mxb_paged_attention_decode_quantized_supported(int head_dim, int hea
 // put together and projected by one kernel, as mxb_paged_attention_decode_project does.
 // settled: with chained launches on, the positions ahead of each token's own were
 // written by launches before the last one, and may be fetched while that one runs.
-MXB_API int mxb_paged_attention_decode_quantized(const void* q, const void* codes, const float* scales, int kind, void* out, float* partial,
-                                                 const int* block_tables, int max_pages, const int* row_token, const int* row_request,
-                                                 const int* positions, int rows, int tokens, int heads, int kv_heads, int head_dim,
-                                                 int page_tokens, int num_pages, int max_splits, int window, int chunk, int keep,
-                                                 float scale, int dtype, const void* w, long long ldw, int hidden, float* summands,
-                                                 const void* gate, long long gate_stride, float softcap, int has_sink, float sink_score,
-                                                 const float* sink_heads, const float* bias_table, int bias_far, int settled,
-                                                 int* status, cudaStream_t stream) {
-  if (rows <= 0) return 0;
-  if (!mxb_paged_attention_decode_quantized_supported(head_dim, heads, kv_heads, dtype) || max_splits <= 0 || page_tokens <= 0 ||
-      num_pages <= 0 || rows > 65535 || (kind != kCodesE4M3 && kind != kCodesInt8) || (bias_table != nullptr && bias_far < 0) ||
-      static_cast<long long>(num_pages) * 2 * kv_heads * page_tokens > 0x7fffffffLL)
+MXB_API int mxb_paged_attention_decode_quantized(const void* call, int bytes, cudaStream_t stream) {
+  if (bytes != static_cast<int>(sizeof(QuantizedDecodeCall))) return static_cast<int>(cudaErrorInvalidValue);
+  const QuantizedDecodeCall& c = *static_cast<const QuantizedDecodeCall*>(call);
+  if (c.rows <= 0) return 0;
+  const int dtype = static_cast<int>(c.dtype), heads = static_cast<int>(c.heads), kv_heads = static_cast<int>(c.kv_heads),
+            head_dim = static_cast<int>(c.head_dim), rows = static_cast<int>(c.rows), tokens = static_cast<int>(c.tokens),
+            max_splits = static_cast<int>(c.max_splits), kind = static_cast<int>(c.kind), window = static_cast<int>(c.window),
+            chunk = static_cast<int>(c.chunk), keep = static_cast<int>(c.keep), has_sink = static_cast<int>(c.has_sink),
+            hidden = static_cast<int>(c.hidden);
+  const float sink_score = static_cast<float>(c.sink_score);
+  if (!quantized_decode_takes(head_dim, heads, kv_heads, dtype) || max_splits <= 0 || c.page_tokens <= 0 ||
+      c.num_pages <= 0 || rows > 65535 || (kind != kCodesE4M3 && kind != kCodesInt8) || (c.bias_table != nullptr && c.bias_far < 0) ||
+      c.num_pages * 2 * kv_heads * c.page_tokens > 0x7fffffffLL)
     return static_cast<int>(cudaErrorInvalidValue);
-  if (w != nullptr && (dtype != kBF16 || hidden <= 0 || !decode_project_takes(head_dim, tokens, w, ldw)))
+  if (c.w != nullptr && (dtype != kBF16 || hidden <= 0 || !decode_project_takes(head_dim, tokens, c.w, c.ldw)))
     return static_cast<int>(cudaErrorInvalidValue);
-  const QuantizedDecode args = {q, static_cast<const uint8_t*>(codes), scales, partial, block_tables, max_pages, row_token, row_request,
-                                positions, heads, kv_heads, head_dim, page_tokens, num_pages, window, chunk, keep, scale, softcap,
-                                ScoreBias{bias_table, bias_far}, settled, status};
+  const QuantizedDecode args = {c.q, static_cast<const uint8_t*>(c.codes), c.scales, c.partial, c.block_tables,
+                                static_cast<int>(c.max_pages), c.row_token, c.row_request, c.positions, heads, kv_heads, head_dim,
+                                static_cast<int>(c.page_tokens), static_cast<int>(c.num_pages), window, chunk, keep,
+                                static_cast<float>(c.scale), static_cast<float>(c.softcap),
+                                ScoreBias{c.bias_table, static_cast<int>(c.bias_far)}, static_cast<int>(c.settled), c.status};
   int slots = 1;
   const cudaError_t e = dtype == kF32 ? launch_quantized_decode<float>(args, kind, rows, max_splits, &slots, stream)
                                       : launch_quantized_decode<__nv_bfloat16>(args, kind, rows, max_splits, &slots, stream);
   if (e != cudaSuccess) return static_cast<int>(e);
-  if (w != nullptr) {
+  if (c.w != nullptr) {
     auto project = head_dim == 64 ? launch_merge_project<64> : launch_merge_project<128>;
-    return static_cast<int>(project(partial, static_cast<const __nv_bfloat16*>(w), ldw, summands, row_token, positions, rows, tokens,
-                                    heads, hidden, max_splits, window, chunk, keep, slots, kSplitKeys, kDecodeMinusHuge,
-                                    static_cast<const __nv_bfloat16*>(gate), gate_stride, has_sink, sink_score, sink_heads, status,
-                                    stream));
+    return static_cast<int>(project(c.partial, static_cast<const __nv_bfloat16*>(c.w), c.ldw, c.summands, c.row_token, c.positions,
+                                    rows, tokens, heads, hidden, max_splits, window, chunk, keep, slots, kSplitKeys, kDecodeMinusHuge,
+                                    static_cast<const __nv_bfloat16*>(c.gate), c.gate_stride, has_sink, sink_score, c.sink_heads,
+                                    c.status, stream));
   }
-  auto merge = [&](auto* target, const auto* gates) {
+  auto merge = [&](auto* target, const auto* gate) {
     using T = std::remove_pointer_t<decltype(target)>;
     return static_cast<int>(launch_chained(paged_attention_merge_kernel<T>, dim3(rows, heads),
                                            dim3(head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256)), 0, stream,
-                                           static_cast<const float*>(partial), target, row_token, positions, rows, heads, head_dim,
-                                           max_splits, window, chunk, keep, slots, gates, gate_stride, has_sink, sink_score,
-                                           sink_heads, status));
+                                           static_cast<const float*>(c.partial), target, c.row_token, c.positions, rows, heads, head_dim,
+                                           max_splits, window, chunk, keep, slots, gate, c.gate_stride, has_sink, sink_score,
+                                           c.sink_heads, c.status));
   };
-  if (dtype == kF32) return merge(static_cast<float*>(out), static_cast<const float*>(gate));
-  return merge(static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(gate));
+  if (dtype == kF32) return merge(static_cast<float*>(c.out), static_cast<const float*>(c.gate));
+  return merge(static_cast<__nv_bfloat16*>(c.out), static_cast<const __nv_bfloat16*>(c.gate));
 }
 
 // ---------------------------------------------------------------------------

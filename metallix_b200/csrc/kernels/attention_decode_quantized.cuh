@@ -458,8 +458,10 @@ static int quantized_slots(int pairs, int max_splits, int resident) {
 template <typename T, int KIND, int HD>
 static cudaError_t launch_quantized_mma(const QuantizedDecode& args, dim3 grid, cudaStream_t stream) {
   auto kernel = args.bias.table != nullptr ? quantized_decode_mma_kernel<T, KIND, HD, true> : quantized_decode_mma_kernel<T, KIND, HD, false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, QuantTile<HD>::kShared);
-  if (e != cudaSuccess) return e;
+  if (QuantTile<HD>::kShared > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, QuantTile<HD>::kShared);
+    if (e != cudaSuccess) return e;
+  }
   return launch_chained(kernel, grid, dim3(kDecodeThreads), QuantTile<HD>::kShared, stream, args);
 }
 

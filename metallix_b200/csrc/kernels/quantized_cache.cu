@@ -141,7 +141,221 @@ __global__ void __launch_bounds__(256) store_quantized_kernel(const StoreArgs a)
   if (threadIdx.x == 0) a.scales[pool_row] = row.scale;
 }
 
-// Pages back into the compute type: block (page of the table, request). The
+// The same for heads of 64, 128 and 256 values with rotations of whole eights of
+// pairs: a lane holds two runs of eight values that contain their own rotation
+// partners, HD / 16 lanes make up a head, and sums and maxima run over a head's
+// lanes. Run A of lane s starts at 8 s and run B half the rotated values
+// further (rotations of halves), or they are neighbours (neighbouring pairs, and
+// the values behind the rotated ones); either way the lane needs the cosines
+// 8 s ... 8 s + 7. Bound by its loads and stores.
+template <typename T, int KIND, int HD>
+__global__ void __launch_bounds__(256) store_quantized_lanes_kernel(const StoreArgs a) {
+  constexpr int LANES = HD / 16, HEADS = 32 / LANES;   // lanes of a head, heads of a warp
+  constexpr int WORDS = 8 * sizeof(T) / 16;            // 16-byte words of a run
+  chain_release();
+  // Up to chain_wait(): only the step's integers and what no kernel of a step writes.
+  const int lane = threadIdx.x & 31, sub = lane % LANES;
+  const unsigned per_token = a.heads + 2 * a.kv_heads, total = static_cast<unsigned>(a.tokens) * per_token;   // below 2^31: the launcher sees to it
+  const unsigned item = (blockIdx.x * 8u + (threadIdx.x >> 5)) * HEADS + lane / LANES;
+  bool active = item < total;   // lanes without work stay to the end: the others exchange values with their warp
+  const int t = active ? static_cast<int>(item / per_token) : 0;
+  const int h = active ? static_cast<int>(item - static_cast<unsigned>(t) * per_token) : 0;
+  const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv_heads;
+  const int kv = is_q ? 0 : (is_k ? h - a.heads : h - a.heads - a.kv_heads);
+  const T* src = is_q   ? static_cast<const T*>(a.q_in) + t * a.q_stride + static_cast<long long>(h) * HD
+                 : is_k ? static_cast<const T*>(a.k_in) + t * a.k_stride + static_cast<long long>(kv) * HD
+                        : static_cast<const T*>(a.v_in) + t * a.v_stride + static_cast<long long>(kv) * HD;
+  size_t pool_row = 0;
+  if (is_q) {
+    if (a.q_out == nullptr) active = false;
+  } else if (active) {
+    const int slot = a.slots[t], page = slot / a.page_tokens;
+    if (slot < 0) {
+      active = false;
+    } else if (page >= a.num_pages) {
+      if (sub == 0) atomicOr(a.status, kStatusBadSlot);
+      active = false;
+    } else {
+      pool_row = ((static_cast<size_t>(page) * 2 + (is_k ? 0 : 1)) * a.kv_heads + kv) * a.page_tokens + (slot - page * a.page_tokens);
+    }
+  }
+  const bool worked = is_q || is_k;   // values are stored as projected
+  const int half = a.rotary_dim >> 1;
+  const bool rotates = a.cos_table != nullptr, turns = rotates && worked && 16 * sub < a.rotary_dim;
+  // runs of halves, where the lane's values are rotated so; else neighbours
+  const bool apart = rotates && !a.interleaved && 16 * sub < a.rotary_dim;
+  const int at_a = apart ? 8 * sub : 16 * sub, at_b = apart ? half + 8 * sub : 16 * sub + 8;
+  const float* weight = is_q ? a.q_weight : (is_k ? a.k_weight : nullptr);
+  float gain[16], c[8], sn[8];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) gain[j] = 1.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) { c[j] = 1.0f; sn[j] = 0.0f; }
+  auto floats = [](float* to, const float* from) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const float4 x = reinterpret_cast<const float4*>(from)[w];
+      to[4 * w] = x.x; to[4 * w + 1] = x.y; to[4 * w + 2] = x.z; to[4 * w + 3] = x.w;
+    }
+  };
+  if (active && weight != nullptr) {
+    if (a.row_sums != nullptr) weight += static_cast<size_t>(is_q ? h : kv) * HD;
+    floats(gain, weight + at_a);
+    floats(gain + 8, weight + at_b);
+  }
+  float factor = 1.0f;
+  if (active && worked && (rotates || a.q_factors != nullptr)) {
+    const int pos = a.positions[t];
+    bool there = true;
+    if (rotates) there = pos >= 0 && pos < a.table_positions;
+    if (turns) {
+      const size_t row = static_cast<size_t>(there ? pos : 0) * half + 8 * sub;
+      floats(c, a.cos_table + row);
+      floats(sn, a.sin_table + row);
+    }
+    if (is_q && a.q_factors != nullptr) {
+      const bool known = pos >= 0 && pos < a.factor_positions;
+      factor = a.q_factors[known ? pos : 0];
+      there = there && known;
+    }
+    if (!there && sub == 0) atomicOr(a.status, kStatusBadSlot);
+  }
+  chain_wait();
+  src = behind_wait(src);   // written by the kernel ahead of this one
+  alignas(16) T in[16] = {};
+  if (active) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      reinterpret_cast<uint4*>(in)[w] = reinterpret_cast<const uint4*>(src + at_a)[w];
+      reinterpret_cast<uint4*>(in)[WORDS + w] = reinterpret_cast<const uint4*>(src + at_b)[w];
+    }
+  }
+  float x[16], sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    x[j] = to_float(in[j]);
+    sum += x[j] * x[j];
+  }
+  if (a.q_weight != nullptr || a.k_weight != nullptr) {   // the same for the whole launch
+#pragma unroll
+    for (int offset = LANES / 2; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+    if (weight != nullptr) {
+      const float mean = a.row_sums != nullptr ? behind_wait(a.row_sums)[2 * t + (is_k ? 1 : 0)] : sum / static_cast<float>(HD);
+      const float scale = rsqrtf(mean + a.eps);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = x[j] * scale * gain[j];
+    }
+  }
+  if (turns) {
+    if (a.interleaved) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float lo = x[2 * j], hi = x[2 * j + 1];
+        x[2 * j] = lo * c[j] - hi * sn[j];
+        x[2 * j + 1] = hi * c[j] + lo * sn[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float lo = x[j], hi = x[8 + j];
+        x[j] = lo * c[j] - hi * sn[j];
+        x[8 + j] = hi * c[j] + lo * sn[j];
+      }
+    }
+  }
+  uint32_t largest = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) largest = max(largest, magnitude_bits(x[j]));
+#pragma unroll
+  for (int offset = LANES / 2; offset > 0; offset >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
+  if (!active) return;
+  if (is_q) {
+    alignas(16) T out[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) out[j] = from_float<T>(x[j] * factor);
+    T* dst = static_cast<T*>(a.q_out) + (static_cast<size_t>(t) * a.heads + h) * HD;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      reinterpret_cast<uint4*>(dst + at_a)[w] = reinterpret_cast<const uint4*>(out)[w];
+      reinterpret_cast<uint4*>(dst + at_b)[w] = reinterpret_cast<const uint4*>(out)[WORDS + w];
+    }
+    return;
+  }
+  const RowScale row = row_scale<KIND>(largest);
+  uint32_t words[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    words[w] = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) words[w] |= code_of<KIND>(x[4 * w + j], row) << (8 * j);
+  }
+  uint8_t* dst = a.codes + pool_row * HD;
+  *reinterpret_cast<uint2*>(dst + at_a) = make_uint2(words[0], words[1]);
+  *reinterpret_cast<uint2*>(dst + at_b) = make_uint2(words[2], words[3]);
+  if (sub == 0) a.scales[pool_row] = row.scale;
+}
+
+// Sixteen codes as values of T.
+template <typename T, int KIND> __device__ __forceinline__ void code_values(const uint4& word, float scale, T* out) {
+  const uint32_t w[4] = {word.x, word.y, word.z, word.w};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) out[i] = from_float<T>(code_value<KIND>((w[i >> 2] >> (8 * (i & 3))) & 0xffu) * scale);
+}
+
+// Pages back into the compute type, for rows of whole 16-byte pieces: a page's
+// codes are one run of memory, and so are its values, so a block takes
+// kReadPieces pieces of one page at a time, each thread all its loads in flight
+// before the first store. Block (x, request) takes the items x, x + gridDim.x, ...
+// of the request's walk over the pages that are seen.
+constexpr int kReadThreads = 256, kReadDepth = 4, kReadPieces = kReadThreads * kReadDepth;
+constexpr int kReadBlocks = 8 * 148 * 8;   // of a launch, at most (or one a request): eight rounds of what is resident
+
+template <typename T, int KIND>
+__global__ void __launch_bounds__(kReadThreads)
+read_cache_pieces_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out,
+                         const int* __restrict__ block_tables, int max_pages, const int* __restrict__ row_request,
+                         const int* __restrict__ first, const int* __restrict__ last, int kv_heads, int head_dim, int page_tokens,
+                         int num_pages, int window, int chunk, int keep, int* status) {
+  const int row = blockIdx.y, end = last[row];
+  if (end < 0) return;
+  const KeyWalk walk = key_walk(min(first_visible_key(max(first[row], 0), window, chunk), end), end, keep, page_tokens);
+  const int per_row = head_dim >> 4, rows = 2 * kv_heads * page_tokens, pieces = rows * per_row;
+  const int per_page = (pieces + kReadPieces - 1) / kReadPieces;
+  const int* table = block_tables + static_cast<size_t>(row_request[row]) * max_pages;
+  for (int item = blockIdx.x; item < walk.count * per_page; item += gridDim.x) {
+    const int step = item / per_page, slot = walk.tile(step), piece0 = (item - step * per_page) * kReadPieces;
+    const int page = slot < max_pages ? table[slot] : -1;
+    if (page < 0 || page >= num_pages) {
+      if (threadIdx.x == 0) atomicOr(status, kStatusBadPage);
+      continue;
+    }
+    const int seen = end - slot * page_tokens + 1;   // rows of the page up to the last position
+    const size_t base = static_cast<size_t>(page) * rows;
+    const uint4* src = reinterpret_cast<const uint4*>(codes + base * head_dim);
+    uint4 held[kReadDepth];
+    float scale[kReadDepth];
+    bool there[kReadDepth];
+#pragma unroll
+    for (int j = 0; j < kReadDepth; ++j) {
+      const int piece = piece0 + j * kReadThreads + threadIdx.x, line = piece / per_row;
+      there[j] = piece < pieces && (seen >= page_tokens || line % page_tokens < seen);
+      held[j] = there[j] ? src[piece] : make_uint4(0u, 0u, 0u, 0u);
+      scale[j] = there[j] ? scales[base + line] : 0.0f;
+    }
+    T* dst = out + base * head_dim;
+#pragma unroll
+    for (int j = 0; j < kReadDepth; ++j) {
+      if (!there[j]) continue;
+      alignas(16) T values[16];
+      code_values<T, KIND>(held[j], scale[j], values);
+      uint4* to = reinterpret_cast<uint4*>(dst + static_cast<size_t>(piece0 + j * kReadThreads + threadIdx.x) * 16);
+#pragma unroll
+      for (int w = 0; w < static_cast<int>(sizeof(T)); ++w) to[w] = reinterpret_cast<const uint4*>(values)[w];
+    }
+  }
+}
+
+// The general form, a code at a time: block (page of the table, request). The
 // rows up to the request's last position are written, everything else of
 // `out` stays as it is.
 template <typename T, int KIND>
@@ -178,38 +392,72 @@ static bool pool_fits(int num_pages, int kv_heads, int page_tokens) {
          static_cast<long long>(num_pages) * 2 * kv_heads * page_tokens <= 0x7fffffffLL;
 }
 
+// What mxb_store_quantized is asked for, 8 bytes a field.
+struct StoreCall {
+  const void *q_in, *k_in, *v_in;
+  void *q_out, *codes;
+  float* scales;
+  const int *slots, *positions;
+  const float *q_weight, *k_weight, *cos_table, *sin_table;
+  float* row_sums;
+  const float* q_factors;
+  int* status;
+  long long q_stride, k_stride, v_stride, kind, dtype, table_positions, rotary_dim, interleaved, norm_scope, tokens, heads, kv_heads,
+      head_dim, page_tokens, num_pages, factor_positions;
+  double eps;
+};
+
 // The norm and rotation of a step's queries and keys, queries to q_out, keys and
 // values into the pool as codes at `slots` (negative: not written). row_sums:
 // float32 scratch of 2 * tokens values for norm_scope 1 (a norm over a token's
 // whole projection; weights [heads * head_dim] and [kv_heads * head_dim]).
-MXB_API int mxb_store_quantized(const void* q_in, const void* k_in, const void* v_in, long long q_stride, long long k_stride,
-                                long long v_stride, void* q_out, void* codes, float* scales, int kind, const int* slots,
-                                const int* positions, const float* q_weight, const float* k_weight, const float* cos_table,
-                                const float* sin_table, int table_positions, int rotary_dim, int interleaved, int norm_scope,
-                                float* row_sums, int tokens, int heads, int kv_heads, int head_dim, int page_tokens, int num_pages,
-                                float eps, int dtype, const float* q_factors, int factor_positions, int* status,
-                                cudaStream_t stream) {
-  if (tokens <= 0) return 0;
-  if (codes == nullptr || scales == nullptr || slots == nullptr || !pool_fits(num_pages, kv_heads, page_tokens) || head_dim <= 0 ||
-      head_dim > 512 || heads < 0 || heads + 2 * kv_heads > 65535 || rotary_dim < 0 || rotary_dim > head_dim || (rotary_dim & 1) ||
-      (dtype != kF32 && dtype != kBF16) || (kind != kCodesE4M3 && kind != kCodesInt8) || (norm_scope == 1 && row_sums == nullptr))
+MXB_API int mxb_store_quantized(const void* call, int bytes, cudaStream_t stream) {
+  if (bytes != static_cast<int>(sizeof(StoreCall))) return static_cast<int>(cudaErrorInvalidValue);
+  const StoreCall& c = *static_cast<const StoreCall*>(call);
+  if (c.tokens <= 0) return 0;
+  const int kind = static_cast<int>(c.kind), dtype = static_cast<int>(c.dtype), tokens = static_cast<int>(c.tokens),
+            heads = static_cast<int>(c.heads), kv_heads = static_cast<int>(c.kv_heads), head_dim = static_cast<int>(c.head_dim),
+            page_tokens = static_cast<int>(c.page_tokens), num_pages = static_cast<int>(c.num_pages);
+  if (c.codes == nullptr || c.scales == nullptr || c.slots == nullptr || !pool_fits(num_pages, kv_heads, page_tokens) || head_dim <= 0 ||
+      head_dim > 512 || heads < 0 || heads + 2 * kv_heads > 65535 || c.rotary_dim < 0 || c.rotary_dim > head_dim || (c.rotary_dim & 1) ||
+      (dtype != kF32 && dtype != kBF16) || (kind != kCodesE4M3 && kind != kCodesInt8) || (c.norm_scope == 1 && c.row_sums == nullptr))
     return static_cast<int>(cudaErrorInvalidValue);
-  if (norm_scope == 1 && (q_weight != nullptr || k_weight != nullptr)) {
+  if (c.norm_scope == 1 && (c.q_weight != nullptr || c.k_weight != nullptr)) {
     const dim3 grid(tokens, 2);
     if (dtype == kF32)
-      projection_squares_kernel<float><<<grid, 256, 0, stream>>>(static_cast<const float*>(q_in), static_cast<const float*>(k_in), q_stride,
-                                                                  k_stride, heads * head_dim, kv_heads * head_dim, row_sums);
+      projection_squares_kernel<float><<<grid, 256, 0, stream>>>(static_cast<const float*>(c.q_in), static_cast<const float*>(c.k_in), c.q_stride,
+                                                                  c.k_stride, heads * head_dim, kv_heads * head_dim, c.row_sums);
     else
       projection_squares_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(
-          static_cast<const __nv_bfloat16*>(q_in), static_cast<const __nv_bfloat16*>(k_in), q_stride, k_stride, heads * head_dim,
-          kv_heads * head_dim, row_sums);
+          static_cast<const __nv_bfloat16*>(c.q_in), static_cast<const __nv_bfloat16*>(c.k_in), c.q_stride, c.k_stride,
+          heads * head_dim, kv_heads * head_dim, c.row_sums);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  const StoreArgs args = {q_in, k_in, v_in, q_stride, k_stride, v_stride, q_out, static_cast<uint8_t*>(codes), scales, slots, positions,
-                          q_weight, k_weight, cos_table, sin_table, table_positions, rotary_dim, interleaved,
-                          norm_scope == 1 ? row_sums : nullptr, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, eps,
-                          q_factors, factor_positions, status};
+  const StoreArgs args = {c.q_in, c.k_in, c.v_in, c.q_stride, c.k_stride, c.v_stride, c.q_out, static_cast<uint8_t*>(c.codes), c.scales,
+                          c.slots, c.positions, c.q_weight, c.k_weight, c.cos_table, c.sin_table, static_cast<int>(c.table_positions),
+                          static_cast<int>(c.rotary_dim), static_cast<int>(c.interleaved), c.norm_scope == 1 ? c.row_sums : nullptr,
+                          tokens, heads, kv_heads, head_dim, page_tokens, num_pages, static_cast<float>(c.eps), c.q_factors,
+                          static_cast<int>(c.factor_positions), c.status};
+  // The lanes' form: 16-byte accesses throughout, runs of eight that hold their rotation partners.
+  const int element = dtype == kF32 ? 4 : 2;
+  auto aligned = [&](const void* p, long long stride) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride * element) % 16 == 0);
+  };
+  const long long items = static_cast<long long>(tokens) * (heads + 2 * kv_heads);
+  if ((head_dim == 64 || head_dim == 128 || head_dim == 256) && items < 0x7fffffffLL && c.rotary_dim % 16 == 0 &&
+      aligned(c.q_in, c.q_stride) && aligned(c.k_in, c.k_stride) && aligned(c.v_in, c.v_stride) && aligned(c.q_out, 0) &&
+      aligned(c.codes, 0) && aligned(c.q_weight, 0) && aligned(c.k_weight, 0) && aligned(c.cos_table, 0) && aligned(c.sin_table, 0)) {
+    const int heads_per_block = 8 * (32 / (head_dim / 16));
+    const dim3 grid(static_cast<unsigned>((items + heads_per_block - 1) / heads_per_block));
+    auto launch = [&](auto kernel) { return static_cast<int>(launch_chained(kernel, grid, dim3(256), 0, stream, args)); };
+#define BY_SIZE(T, KIND) (head_dim == 64    ? launch(store_quantized_lanes_kernel<T, KIND, 64>)  \
+                          : head_dim == 128 ? launch(store_quantized_lanes_kernel<T, KIND, 128>) \
+                                            : launch(store_quantized_lanes_kernel<T, KIND, 256>))
+    if (dtype == kF32) return kind == kCodesInt8 ? BY_SIZE(float, kCodesInt8) : BY_SIZE(float, kCodesE4M3);
+    return kind == kCodesInt8 ? BY_SIZE(__nv_bfloat16, kCodesInt8) : BY_SIZE(__nv_bfloat16, kCodesE4M3);
+#undef BY_SIZE
+  }
   auto launch = [&](auto kernel) {
     kernel<<<dim3(tokens, heads + 2 * kv_heads), 256, head_dim * sizeof(float), stream>>>(args);
     return static_cast<int>(cudaGetLastError());
@@ -220,23 +468,50 @@ MXB_API int mxb_store_quantized(const void* q_in, const void* k_in, const void* 
                             : launch(store_quantized_kernel<__nv_bfloat16, kCodesE4M3>);
 }
 
+// What mxb_read_cache is asked for, 8 bytes a field.
+struct ReadCall {
+  const void* codes;
+  const float* scales;
+  void* out;
+  const int *block_tables, *row_request, *first, *last;
+  int* status;
+  long long kind, dtype, max_pages, rows, kv_heads, head_dim, page_tokens, num_pages, window, chunk, keep;
+};
+
 // For each i < rows: the pages of row row_request[i] of the block tables that a
 // query at position first[i] or later sees (window, chunk, keep as in the
 // attention kernels), up to position last[i], from the pool into `out`, which
 // has the pool's layout [pages, 2, kv_heads, page_tokens, head_dim] in `dtype`.
-MXB_API int mxb_read_cache(const void* codes, const float* scales, int kind, void* out, int dtype, const int* block_tables, int max_pages,
-                           const int* row_request, const int* first, const int* last, int rows, int kv_heads, int head_dim,
-                           int page_tokens, int num_pages, int window, int chunk, int keep, int* status, cudaStream_t stream) {
-  if (rows <= 0 || max_pages <= 0) return 0;
+MXB_API int mxb_read_cache(const void* call, int bytes, cudaStream_t stream) {
+  if (bytes != static_cast<int>(sizeof(ReadCall))) return static_cast<int>(cudaErrorInvalidValue);
+  const ReadCall& c = *static_cast<const ReadCall*>(call);
+  if (c.rows <= 0 || c.max_pages <= 0) return 0;
+  const int kind = static_cast<int>(c.kind), dtype = static_cast<int>(c.dtype), rows = static_cast<int>(c.rows),
+            kv_heads = static_cast<int>(c.kv_heads), head_dim = static_cast<int>(c.head_dim), max_pages = static_cast<int>(c.max_pages),
+            page_tokens = static_cast<int>(c.page_tokens), num_pages = static_cast<int>(c.num_pages);
+  void* out = c.out;
   if (rows > 65535 || !pool_fits(num_pages, kv_heads, page_tokens) || head_dim <= 0 || head_dim > 512 ||
       (dtype != kF32 && dtype != kBF16) || (kind != kCodesE4M3 && kind != kCodesInt8))
     return static_cast<int>(cudaErrorInvalidValue);
+  const bool by_pieces = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(c.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  // A block an item where tables are short; wide tables of short contexts (a captured step's) walk with a stride instead.
+  const long long items = static_cast<long long>(max_pages) * ((2LL * kv_heads * page_tokens * (head_dim / 16) + kReadPieces - 1) / kReadPieces);
+  const long long most = kReadBlocks / rows > 0 ? kReadBlocks / rows : 1;
+  const dim3 grid(static_cast<unsigned>(!by_pieces ? max_pages : (items < most ? items : most)), rows);
   auto launch = [&](auto kernel, auto* target) {
-    kernel<<<dim3(max_pages, rows), 256, 0, stream>>>(static_cast<const uint8_t*>(codes), scales, target, block_tables, max_pages,
-                                                     row_request, first, last, kv_heads, head_dim, page_tokens, num_pages, window,
-                                                     chunk, keep, status);
+    kernel<<<grid, kReadThreads, 0, stream>>>(static_cast<const uint8_t*>(c.codes), c.scales, target, c.block_tables,
+                                                     max_pages, c.row_request, c.first, c.last, kv_heads, head_dim, page_tokens,
+                                                     num_pages, static_cast<int>(c.window), static_cast<int>(c.chunk),
+                                                     static_cast<int>(c.keep), c.status);
     return static_cast<int>(cudaGetLastError());
   };
+  if (by_pieces) {
+    if (dtype == kF32)
+      return kind == kCodesInt8 ? launch(read_cache_pieces_kernel<float, kCodesInt8>, static_cast<float*>(out))
+                                : launch(read_cache_pieces_kernel<float, kCodesE4M3>, static_cast<float*>(out));
+    return kind == kCodesInt8 ? launch(read_cache_pieces_kernel<__nv_bfloat16, kCodesInt8>, static_cast<__nv_bfloat16*>(out))
+                              : launch(read_cache_pieces_kernel<__nv_bfloat16, kCodesE4M3>, static_cast<__nv_bfloat16*>(out));
+  }
   if (dtype == kF32)
     return kind == kCodesInt8 ? launch(read_cache_kernel<float, kCodesInt8>, static_cast<float*>(out))
                               : launch(read_cache_kernel<float, kCodesE4M3>, static_cast<float*>(out));

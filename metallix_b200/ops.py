@@ -7,6 +7,7 @@ another implementation. Kernels run on torch's current CUDA stream.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -15,6 +16,7 @@ from .csrc import build
 
 F32, BF16 = 0, 1
 _CODES = {torch.float32: F32, torch.bfloat16: BF16}
+_COMPUTE = tuple(_CODES)
 
 STATUS_BITS = {1: "a token id outside the vocabulary", 2: "a cache slot or position outside its table",
                4: "a block-table entry outside the page pool", 8: "non-finite logits",
@@ -25,7 +27,7 @@ class KernelError(RuntimeError):
     pass
 
 
-_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_P, _I, _L, _F, _C = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_char_p
 _SIGNATURES = {
     "mxb_embed": [_P, _P, _I, _P, _I, _I, _I, _F, _P, _P],
     "mxb_rmsnorm": [_P, _I, _P, _I, _P, _P, _I, _I, _F, _P],
@@ -90,12 +92,9 @@ _SIGNATURES = {
     "mxb_plain_activation": [_P, _P, _L, _I, _I, _P],
     "mxb_paged_attention_decode": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
                                    _F, _I, _P, _L, _F, _I, _F, _P, _P, _I, _P, _P],
-    "mxb_paged_attention_decode_quantized_supported": [_I, _I, _I, _I],
-    "mxb_paged_attention_decode_quantized": [_P, _P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
-                                             _F, _I, _P, _L, _I, _P, _P, _L, _F, _I, _F, _P, _P, _I, _I, _P, _P],
-    "mxb_store_quantized": [_P, _P, _P, _L, _L, _L, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _I, _I, _I, _I, _I,
-                            _F, _I, _P, _I, _P, _P],
-    "mxb_read_cache": [_P, _P, _I, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "mxb_paged_attention_decode_quantized": [_C, _I, _P],
+    "mxb_store_quantized": [_C, _I, _P],
+    "mxb_read_cache": [_C, _I, _P],
     "mxb_postnorm_add_rmsnorm": [_P, _P, _I, _I, _P, _F, _P, _I, _P, _F, _I, _I, _P],
     "mxb_sigmoid_gate": [_P, _P, _P, _L, _L, _L, _I, _I, _I, _P],
     "mxb_softcap": [_P, _F, _L, _P],
@@ -174,13 +173,14 @@ def _call(name: str, *args) -> None:
         raise KernelError(f"{name} failed to launch: CUDA error {code}")
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _stream() -> int:
     """The current stream's handle; this runs once per launch, so it takes the short way."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(_current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -1318,13 +1318,21 @@ class QuantizedPool:
     __slots__ = ("codes", "scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        self.codes, self.scales = codes, scales
+        if not (type(codes) is type(scales) is torch.Tensor and codes.dtype in _CODE_KINDS and scales.dtype is torch.float32
+                and codes.is_contiguous() and scales.is_contiguous() and codes.dim() == 5 and codes.shape[1] == 2
+                and scales.shape == codes.shape[:4] and codes.is_cuda and codes.get_device() == scales.get_device()
+                and scales.numel() < 1 << 31):
+            self._refuse()
+
+    def _refuse(self) -> None:
+        codes, scales = self.codes, self.scales
         _check(codes, "codes", tuple(_CODE_KINDS), 5)
         _check(scales, "scales", (torch.float32,), 4)
         _need(codes.shape[1] == 2, "codes must be [pages, 2, kv_heads, page_tokens, head_dim]")
         _need(scales.shape == codes.shape[:4], "one scale per row: scales must be [pages, 2, kv_heads, page_tokens]")
         _need(scales.device == codes.device, "codes and scales are on different devices")
         _need(scales.numel() < 1 << 31, f"a pool of {scales.numel()} rows: the kernels count rows in 31 bits")
-        self.codes, self.scales = codes, scales
 
     @classmethod
     def zeros(cls, pages: int, kv_heads: int, page_tokens: int, head_dim: int, codes: str = "fp8",
@@ -1343,12 +1351,34 @@ class QuantizedPool:
         return _CODE_KINDS[self.codes.dtype]
 
 
-def _on_current_device(**tensors) -> None:
+def _all_on(device: int, *tensors) -> bool:
+    """Whether all the tensors (those that are not None) are on CUDA device ``device``."""
+    for tensor in tensors:
+        if tensor is not None and tensor.get_device() != device:
+            return False
+    return True
+
+
+def _on_current_device(*tensors) -> None:
     """The kernels run on the current device's current stream: everything has to be there."""
-    current = torch.cuda.current_device()
-    for name, tensor in tensors.items():
-        _need(tensor is None or tensor.device.index == current,
-              f"{name} is on another device than the current one (cuda:{current})")
+    current = _current_device()
+    if not _all_on(current, *tensors):
+        raise KernelError(f"a tensor is on another device than the current one (cuda:{current})")
+
+
+def _int_lists(dims: int, *tensors) -> bool:
+    """Whether all are contiguous int32 tensors of so many dimensions."""
+    for tensor in tensors:
+        if not (isinstance(tensor, torch.Tensor) and tensor.dtype is torch.int32 and tensor.dim() == dims
+                and tensor.is_contiguous() and tensor.is_cuda):
+            return False
+    return True
+
+
+# The calls' fields, in the order of the structs of the same names in csrc/kernels: pointers and whole numbers, then doubles.
+_READ_CALL = struct.Struct("=19q")
+_STORE_CALL = struct.Struct("=31qd")
+_QUANTIZED_DECODE_CALL = struct.Struct("=35q3d")
 
 
 def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tensor, row_request: torch.Tensor,
@@ -1361,22 +1391,27 @@ def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tenso
     block tables serve it; rows that are not read stay as they are. A negative
     ``last`` reads nothing."""
     _need(isinstance(pool, QuantizedPool), "pool must be a QuantizedPool")
-    _check(out, "out", tuple(_CODES), 5)
-    _need(out.shape == pool.shape, "out must have the pool's shape")
-    _check(block_tables, "block_tables", (torch.int32,), 2)
-    for name, tensor in (("row_request", row_request), ("first", first), ("last", last)):
-        _check(tensor, name, (torch.int32,), 1)
-    rows = row_request.numel()
-    _need(first.numel() == rows and last.numel() == rows, "row lists differ in length")
-    _need(rows <= 65535, f"{rows} rows in one call; up to 65535")
-    num_pages, _, kv_heads, page_tokens, head_dim = pool.shape
-    _need(head_dim <= 512, f"head_dim {head_dim} is beyond 512")
-    _on_current_device(pool=pool.codes, out=out, block_tables=block_tables, row_request=row_request, first=first, last=last)
-    if rows and pool.codes.numel():
-        _call("mxb_read_cache", pool.codes.data_ptr(), pool.scales.data_ptr(), pool.kind, out.data_ptr(), _CODES[out.dtype],
-              block_tables.data_ptr(), block_tables.shape[1], row_request.data_ptr(), first.data_ptr(), last.data_ptr(), rows,
-              kv_heads, head_dim, page_tokens, num_pages, int(window or 0), int(chunk or 0), _kept(keep),
-              status_word(out.device).data_ptr(), _stream())
+    codes = pool.codes
+    shape = codes.shape
+    rows = row_request.numel() if isinstance(row_request, torch.Tensor) else 0
+    if not (isinstance(out, torch.Tensor) and out.dtype in _CODES and out.shape == shape and out.is_contiguous() and _int_lists(2, block_tables)
+            and _int_lists(1, row_request, first, last) and first.numel() == last.numel() == rows <= 65535 and shape[4] <= 512):
+        _check(out, "out", tuple(_CODES), 5)
+        _need(out.shape == shape, "out must have the pool's shape")
+        _check(block_tables, "block_tables", (torch.int32,), 2)
+        for name, tensor in (("row_request", row_request), ("first", first), ("last", last)):
+            _check(tensor, name, (torch.int32,), 1)
+        _need(first.numel() == rows and last.numel() == rows, "row lists differ in length")
+        _need(rows <= 65535, f"{rows} rows in one call; up to 65535")
+        _need(shape[4] <= 512, f"head_dim {shape[4]} is beyond 512")
+    _on_current_device(codes, out, block_tables, row_request, first, last)
+    if rows and codes.numel():
+        num_pages, _, kv_heads, page_tokens, head_dim = shape
+        call = _READ_CALL.pack(
+            codes.data_ptr(), pool.scales.data_ptr(), out.data_ptr(), block_tables.data_ptr(), row_request.data_ptr(),
+            first.data_ptr(), last.data_ptr(), status_word(out.device).data_ptr(), _CODE_KINDS[codes.dtype], _CODES[out.dtype],
+            block_tables.shape[1], rows, kv_heads, head_dim, page_tokens, num_pages, window or 0, chunk or 0, _kept(keep))
+        _call("mxb_read_cache", call, len(call), _stream())
     return out
 
 
@@ -1442,17 +1477,19 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
     if q_factors is not None:
         _check(q_factors, "q_factors", (torch.float32,), 1)
     if quantized:
-        _need(head_dim <= 512 and heads + 2 * kv_heads <= 65535, f"{heads} + 2 x {kv_heads} heads of {head_dim} values")
-        _on_current_device(cache=cache.codes, q=q, k=k, v=v, q_out=q_out, slots=slots, positions=positions, q_weight=q_weight,
-                           k_weight=k_weight, cos=cos, sin=sin, q_factors=q_factors)
+        if head_dim > 512 or heads + 2 * kv_heads > 65535:
+            raise KernelError(f"{heads} + 2 x {kv_heads} heads of {head_dim} values")
+        _on_current_device(cache.codes, q, k, v, q_out, slots, positions, q_weight, k_weight, cos, sin, q_factors)
         projection = norm_scope == "projection" and (q_weight is not None or k_weight is not None)
         sums = torch.empty(2 * tokens, dtype=torch.float32, device=q.device) if projection else None
-        _call("mxb_store_quantized", q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
-              _ptr(q_out), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.kind, slots.data_ptr(), positions.data_ptr(),
-              _ptr(q_weight), _ptr(k_weight), _ptr(cos), _ptr(sin), table_positions, rotary_dim, 1 if interleaved else 0,
-              1 if projection else 0, _ptr(sums), tokens, heads, kv_heads, head_dim, page_tokens, num_pages, float(eps),
-              _CODES[dtype], _ptr(q_factors), q_factors.numel() if q_factors is not None else 0,
-              status_word(q.device).data_ptr(), _stream())
+        call = _STORE_CALL.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_out) or 0, cache.codes.data_ptr(), cache.scales.data_ptr(),
+            slots.data_ptr(), positions.data_ptr(), _ptr(q_weight) or 0, _ptr(k_weight) or 0, _ptr(cos) or 0, _ptr(sin) or 0,
+            _ptr(sums) or 0, _ptr(q_factors) or 0, status_word(q.device).data_ptr(), q.stride(0), k.stride(0), v.stride(0),
+            _CODE_KINDS[cache.codes.dtype], _CODES[dtype], table_positions, rotary_dim, 1 if interleaved else 0,
+            1 if projection else 0, tokens, heads, kv_heads, head_dim, page_tokens, num_pages,
+            q_factors.numel() if q_factors is not None else 0, eps)
+        _call("mxb_store_quantized", call, len(call), _stream())
         return
     _call("mxb_qk_norm_rope_cache", q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0),
           v.stride(0), _ptr(q_out), _ptr(cache), _ptr(slots), positions.data_ptr(), _ptr(q_weight),
@@ -1713,9 +1750,7 @@ def set_decode_resident_blocks(blocks: int, many: int = 2048) -> None:
 
 def quantized_decode_supported(head_dim: int, heads: int, kv_heads: int, dtype: torch.dtype) -> bool:
     """Whether the decode attention takes this head layout over a ``QuantizedPool``."""
-    if dtype not in _CODES:
-        return False
-    return bool(_fn("mxb_paged_attention_decode_quantized_supported")(head_dim, heads, kv_heads, _CODES[dtype]))
+    return dtype in _CODES and 0 < head_dim <= 256 and 0 < kv_heads <= heads and heads % kv_heads == 0
 
 
 def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.Tensor], block_tables: torch.Tensor,
@@ -1725,36 +1760,50 @@ def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.
                       weight: Optional[torch.Tensor], summands: Optional[torch.Tensor]) -> None:
     """The decode attention over a quantized pool, into ``out`` or, with the
     output projection ``weight``, into ``summands``."""
-    _need(softcap >= 0.0, "the cap on the scores cannot be negative")
+    global _split_keys
+    codes, dtype = pool.codes, q.dtype
+    num_pages, _, kv_heads, page_tokens, cache_dim = codes.shape
     tokens, heads, head_dim = q.shape
-    num_pages, _, kv_heads, page_tokens, cache_dim = pool.shape
-    _need(cache_dim == head_dim, f"the pool's rows are {cache_dim} values wide, the queries {head_dim}")
-    _need(quantized_decode_supported(head_dim, heads, kv_heads, q.dtype),
-          f"the decode attention over 8-bit rows does not take head_dim {head_dim} with {heads}/{kv_heads} heads in {q.dtype}")
-    _check(block_tables, "block_tables", (torch.int32,), 2)
-    for name, tensor in (("row_token", row_token), ("row_request", row_request), ("positions", positions)):
-        _check(tensor, name, (torch.int32,), 1)
     rows = row_token.numel()
-    _need(row_request.numel() == rows and positions.numel() == tokens, "row lists do not fit")
-    _need(rows <= 65535, f"{rows} rows in one call; up to 65535")
-    splits = max(1, -(-int(longest_context) // decode_split_keys()))
+    if not (cache_dim == head_dim and quantized_decode_supported(head_dim, heads, kv_heads, dtype) and softcap >= 0.0
+            and _int_lists(2, block_tables) and _int_lists(1, row_token, row_request, positions)
+            and row_request.numel() == rows <= 65535 and positions.numel() == tokens):
+        _need(softcap >= 0.0, "the cap on the scores cannot be negative")
+        _need(cache_dim == head_dim, f"the pool's rows are {cache_dim} values wide, the queries {head_dim}")
+        _need(quantized_decode_supported(head_dim, heads, kv_heads, dtype),
+              f"the decode attention over 8-bit rows does not take head_dim {head_dim} with {heads}/{kv_heads} heads in {dtype}")
+        _check(block_tables, "block_tables", (torch.int32,), 2)
+        for name, tensor in (("row_token", row_token), ("row_request", row_request), ("positions", positions)):
+            _check(tensor, name, (torch.int32,), 1)
+        _need(row_request.numel() == rows and positions.numel() == tokens, "row lists do not fit")
+        _need(rows <= 65535, f"{rows} rows in one call; up to 65535")
+    if _split_keys is None:
+        _split_keys = decode_split_keys()
+    splits = max(1, -(-int(longest_context) // _split_keys))
     need = rows * heads * splits * (head_dim + 2)
     if partial is None:
         partial = torch.empty(need, dtype=torch.float32, device=q.device)
-    _check(partial, "partial", (torch.float32,))
-    _need(partial.numel() >= need, f"partial holds {partial.numel()} values, {need} are needed")
+    elif not (partial.dtype is torch.float32 and partial.is_contiguous() and partial.numel() >= need):
+        _check(partial, "partial", (torch.float32,))
+        _need(partial.numel() >= need, f"partial holds {partial.numel()} values, {need} are needed")
     gate_stride = _gate_stride(gate, q)
-    _on_current_device(cache=pool.codes, q=q, out=out, block_tables=block_tables, row_token=row_token, row_request=row_request,
-                       positions=positions, partial=partial, gate=gate, weight=weight)
+    has_sink, sink_score, sink_heads = _sink(sink, heads)
+    bias_table, bias_far = _score_bias(bias, heads)
+    _on_current_device(codes, q, out, block_tables, row_token, row_request, positions, partial, gate, weight,
+                       sink if sink_heads else None, bias)
     hidden, ldw = (weight.shape[0], weight.stride(0)) if weight is not None else (0, 0)
     if not rows:
         return
-    _call("mxb_paged_attention_decode_quantized", q.data_ptr(), pool.codes.data_ptr(), pool.scales.data_ptr(), pool.kind,
-          _ptr(out), partial.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], row_token.data_ptr(),
-          row_request.data_ptr(), positions.data_ptr(), rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits,
-          int(window or 0), int(chunk or 0), _kept(keep), float(scale), _CODES[q.dtype], _ptr(weight), ldw, hidden,
-          _ptr(summands), _ptr(gate), gate_stride, float(softcap), *_sink(sink, heads), *_score_bias(bias, heads),
-          1 if settled else 0, status_word(q.device).data_ptr(), _stream())
+    call = _QUANTIZED_DECODE_CALL.pack(
+        q.data_ptr(), codes.data_ptr(), pool.scales.data_ptr(), _ptr(out) or 0, partial.data_ptr(), block_tables.data_ptr(),
+        row_token.data_ptr(), row_request.data_ptr(), positions.data_ptr(), _ptr(weight) or 0, _ptr(summands) or 0, _ptr(gate) or 0,
+        sink_heads or 0, bias_table or 0, status_word(q.device).data_ptr(), _CODE_KINDS[codes.dtype], _CODES[dtype],
+        block_tables.shape[1], rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits, window or 0, chunk or 0,
+        _kept(keep), ldw, hidden, gate_stride, has_sink, bias_far, 1 if settled else 0, scale, softcap, sink_score)
+    _call("mxb_paged_attention_decode_quantized", call, len(call), _stream())
+
+
+_split_keys: Optional[int] = None
 
 
 def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
@@ -1783,10 +1832,12 @@ def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
     with chained launches on they may be fetched while that one runs (a cache in
     the compute type is taken to be so)."""
     dtype = q.dtype
-    _need(softcap >= 0.0, "the cap on the scores cannot be negative")
-    _check(q, "q", tuple(_CODES), 3)
+    if not softcap >= 0.0:
+        raise KernelError("the cap on the scores cannot be negative")
+    _check(q, "q", _COMPUTE, 3)
     _check(out, "out", (dtype,), 3)
-    _need(out.shape == q.shape, "out and q differ in shape")
+    if out.shape != q.shape:
+        raise KernelError("out and q differ in shape")
     if isinstance(cache, QuantizedPool):
         _decode_quantized(q, cache, out, block_tables, row_token, row_request, positions, scale, longest_context, window,
                           partial, chunk, gate, softcap, sink, bias, keep, settled, None, None)
