@@ -1340,11 +1340,14 @@ MXB_API int mxb_paged_attention_decode_quantized(const void* call, int bytes, cu
     return static_cast<int>(cudaErrorInvalidValue);
   if (c.w != nullptr && (dtype != kBF16 || hidden <= 0 || !decode_project_takes(head_dim, tokens, c.w, c.ldw)))
     return static_cast<int>(cudaErrorInvalidValue);
+  int page_shift = 0;
+  while ((1LL << page_shift) < c.page_tokens) ++page_shift;
+  if ((1LL << page_shift) != c.page_tokens) page_shift = -1;
   const QuantizedDecode args = {c.q, static_cast<const uint8_t*>(c.codes), c.scales, c.partial, c.block_tables,
                                 static_cast<int>(c.max_pages), c.row_token, c.row_request, c.positions, heads, kv_heads, head_dim,
                                 static_cast<int>(c.page_tokens), static_cast<int>(c.num_pages), window, chunk, keep,
                                 static_cast<float>(c.scale), static_cast<float>(c.softcap),
-                                ScoreBias{c.bias_table, static_cast<int>(c.bias_far)}, static_cast<int>(c.settled), c.status};
+                                ScoreBias{c.bias_table, static_cast<int>(c.bias_far)}, page_shift, static_cast<int>(c.settled), c.status};
   int slots = 1;
   const cudaError_t e = dtype == kF32 ? launch_quantized_decode<float>(args, kind, rows, max_splits, &slots, stream)
                                       : launch_quantized_decode<__nv_bfloat16>(args, kind, rows, max_splits, &slots, stream);
