@@ -133,47 +133,69 @@ quantized_decode_kernel(const QuantizedDecode a) {
 //
 // Halves reach from 2^-24 to 2^16, which powers of two make room for: a head's
 // queries are scaled so that the largest lies at 2^14 (what is lost below is
-// 2^-39 of it), and the weights p_j scale_j so that the largest so far does.
-// With `top` the largest such weight on the running maximum's terms, ref = 2^floor(log2 top),
-// the accumulator holds sum_j (2^14 / ref) p_j scale_j code_j.
+// 2^-39 of it), and the weights p_j scale_j by `up`, so that the largest lies at
+// 2^kQuantTop when they are first looked at and may grow up to 2^15. The same
+// goes for the maximum that the exponentials are taken against: it is found by
+// exchanging values only when a stage's sum or weights outgrow their room, so
+// that most stages exchange nothing. What a warp has gathered is
+//   sum_j 2^(s_j - m) scale_j code_j * up   and   sum_j 2^(s_j - m)
+// for any m, which need not be the maximum.
 //
 // A warp works alone until the end: it takes its 32 keys of a 128-key tile (a
-// stage; for heads of 256, 16 of them), copies their rows into a ring of its own
-// by cp.async, each lane exactly the pieces that it will read itself, and so needs
-// neither a barrier nor a bank's favour: a lane's 16 bytes lie beside its
-// neighbours'. What a lane reads is chosen so that bytes need no transposing:
-//   K: lane (g, t) = (lane / 4, lane % 4) of the key g of eight copies the 16-byte
-//      pieces t, t + 4, ... of that row. Word w of a piece gives both registers
-//      of the B operand of one 16-value step; q's registers follow the same
-//      order of values.
-//   V: lane (g, t) copies 16 bytes at g of the rows of the keys 2t, 2t + 1, 2t + 8,
-//      2t + 9, from which byte pairs of neighbouring keys make the A operand
-//      (o^T = V^T p^T: 16 values of a row by 8 query heads, no row of the tile
-//      wasted). The scores lie where p^T's B operand wants them.
+// stage; for heads of 256, 16 of them) and has their rows brought into a ring of
+// its own by TMA, one box per page and plane with the swizzle that lets its lanes
+// read them without bank conflicts. (Copies of 16 bytes a lane by cp.async kept
+// an SM to 34 GB/s times its clock's share however many were under way and
+// however little else was done: 122 us for 8 requests over 32,000 positions.)
+// What a lane reads is chosen so that bytes need no transposing:
+//   K: lane (g, t) = (lane / 4, lane % 4) reads the 16-byte chunks 2t, 2t + 1 of the
+//      key g of eight (heads of 64: chunk t). Word w of a chunk of the keys g and
+//      g + 8 is the A operand of one 16-value step (scores^T = K q^T: 16 keys by 8
+//      query heads); q's registers follow the same order of values.
+//   V: lane (g, t) reads chunk g of the keys 2t, 2t + 1, 2t + 8, 2t + 9, from which
+//      byte pairs of neighbouring keys make the A operand (o^T = V^T p^T: 16 values
+//      of a row by 8 query heads). p^T's B operand is the scores' tile turned by
+//      movmatrix. No row of either product is wasted.
 //
-// float32 queries are two halves each, 22 bits and the sign of what is left (the
-// second as rows 8..15 of the same product); so are the weights, in a product more.
+// float32 queries are two halves each, 22 bits and the sign of what is left; so
+// are the weights: a second product for either.
 template <int HD> struct QuantTile {
   static constexpr int kKeys = HD == 256 ? 16 : 32;            // of a stage
   static constexpr int kBlocks8 = kKeys / 8;                   // eights of keys
-  static constexpr int kKeyPieces = HD / 64;                   // 16-byte pieces of a key row a lane takes
+  static constexpr int kChunks = HD / 64;                      // 16-byte chunks of a key row a lane takes
   static constexpr int kValueBytes = HD >= 128 ? 16 : HD / 8;  // of a value row a lane takes at once
   static constexpr int kValuePieces = HD / 8 / kValueBytes;
+  static constexpr int kBoxBytes = HD >= 128 ? 128 : HD;       // of a row in one box; heads of 256 lie as two halves
   static constexpr int kRowBytes = kKeys * HD;                 // a stage's keys; its values as many
-  static constexpr int kStageBytes = 2 * kRowBytes + 2 * kKeys * 4;   // keys, values, scales
   static constexpr int kStages = HD == 128 ? 2 : 3;
-  static constexpr int kRing = (kDecodeThreads / 32) * kStages * kStageBytes;
+  static constexpr int kWarpBytes = kStages * 2 * kRowBytes;   // the ring's codes; its scales lie behind all warps' codes
+  static constexpr int kScales = 2 * kKeys;                    // of a stage: keys', values'
+  static constexpr int kRing = (kDecodeThreads / 32) * (kWarpBytes + kStages * kScales * 4);
   static constexpr int kMerge = (kDecodeThreads / 32) * 8 * (HD + 2) * 4;
-  static constexpr int kShared = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kShared = (kRing > kMerge ? kRing : kMerge) + 1024;   // and room to align to the swizzle's period
+  // Where chunk c of row r of a stage lies: the hardware's swizzle of 128-byte rows (64-byte ones for heads of 64).
+  static __device__ __forceinline__ int at(int r, int c) {
+    return HD == 64 ? r * 64 + ((c ^ ((r >> 1) & 3)) << 4) : (c >> 3) * (kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+  }
 };
 
-template <int BYTES> __device__ __forceinline__ void quant_copy(void* dst, const void* src, bool there) {
+__device__ __forceinline__ void quant_copy_scale(float* dst, const float* src, bool there) {
   const uint32_t address = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
-  const int size = there ? BYTES : 0;   // else zeros
-  if (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(address), "l"(src), "r"(size));
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(address), "l"(src), "n"(BYTES), "r"(size));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(address), "l"(src), "r"(there ? 4 : 0));   // else zero
+}
+
+// A pool's codes as [rows, head_dim] bytes, read in boxes of box_rows rows. Encoded anew for every call.
+static bool encode_codes_map(CUtensorMap* map, const void* codes, long long rows, int head_dim, int box_rows) {
+  EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return false;
+  const int box = head_dim >= 128 ? 128 : head_dim;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(head_dim)};
+  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t element_strides[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, boxes, element_strides,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // The four codes of a word as two pairs of halves. Whole numbers: with its sign
@@ -194,9 +216,19 @@ template <int KIND> __device__ __forceinline__ void code_halves(uint32_t word, u
 }
 
 __device__ __forceinline__ void quant_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int kQuantTop = 6;
+constexpr float kQuantLow = -1.0e30f;   // the reference before the first key: any score is far above it
+
+// An 8 x 8 tile of halves, two of a row a lane, turned.
+__device__ __forceinline__ uint32_t turn_tile(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // A pair of float32 numbers as PARTS pairs of halves, largest first.
@@ -221,13 +253,15 @@ template <typename T, int HD> struct QuantBlocks {
 
 template <typename T, int KIND, int HD, bool BIASED>
 __global__ void __launch_bounds__(kDecodeThreads, QuantBlocks<T, HD>::value)
-quantized_decode_mma_kernel(const QuantizedDecode a) {
+quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ QuantizedDecode a) {
   using Tile = QuantTile<HD>;
   constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;
   constexpr int WARPS = kDecodeThreads / 32, STAGES = Tile::kStages, STEPS = HD / 16, KEYS = Tile::kKeys, EIGHTS = Tile::kBlocks8;
   constexpr int HALVES = 32 / KEYS;   // stages of a warp's 32 keys of a tile
   constexpr float kLog2E = 1.4426950408889634f;
-  extern __shared__ __align__(16) unsigned char quant_shared[];
+  extern __shared__ unsigned char quant_raw[];
+  __shared__ __align__(8) uint64_t barriers[WARPS * STAGES];
+  unsigned char* quant_shared = quant_raw + ((1024 - (shared_address(quant_raw) & 1023)) & 1023);
   const bool release_late = gridDim.x * gridDim.y * gridDim.z > QuantBlocks<T, HD>::value * 148u;   // as in the kernels over bfloat16 rows
   if (!release_late) chain_release();
   const int rank = blockIdx.x, slots = gridDim.x, kv = blockIdx.y % a.kv_heads, part = blockIdx.y / a.kv_heads, row = blockIdx.z;
@@ -241,84 +275,85 @@ quantized_decode_mma_kernel(const QuantizedDecode a) {
   const KeyWalk walk = key_walk(first_key, pos, a.keep, kSplitKeys);
   if (rank >= walk.count) return;   // more slots than tiles: the merge skips this one
   const int* table = a.block_tables + static_cast<size_t>(a.row_request[row]) * a.max_pages;
-  unsigned char* ring = quant_shared + warp * (STAGES * Tile::kStageBytes);
+  unsigned char* ring = quant_shared + warp * Tile::kWarpBytes;
+  float* ring_scales = reinterpret_cast<float*>(quant_shared + WARPS * Tile::kWarpBytes) + warp * (STAGES * Tile::kScales);
+  uint64_t* landed = barriers + warp * STAGES;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) barrier_init(&landed[i], 1);
+    barrier_init_fence();
+  }
+  __syncwarp();
 
   // Stage i of the warp: part i % HALVES of its keys of the block's tile i / HALVES.
   const int stages = HALVES * ((walk.count - rank + slots - 1) / slots);
   auto first_of = [&](int i) { return walk.tile(rank + i / HALVES * slots) * kSplitKeys + warp * 32 + i % HALVES * KEYS; };
   auto holds = [&](int key0) { return key0 <= pos && (key0 + KEYS > first_key || key0 < a.keep); };
-  // Pages are a power of two of 8 positions or more, so eight keys lie in one of them. Lanes b, b + 4, ... ask for the page
-  // of eight b of a stage, one stage ahead of the copies, and look at it only then.
-  const int shift = a.page_shift, in_page = a.page_tokens - 1;
-  auto page_of = [&](int i) {
-    const int slot = (first_of(i) + lane % EIGHTS * 8) >> shift;
+  auto wanted = [&](int key, int keys) { return key <= pos && (key + keys > first_key || key < a.keep); };
+  // Pages are a power of two of 8 positions or more: a box is a page's rows of one plane, or of a stage where a page has more.
+  // Lane n has box n fetched (keys' boxes, then values'; for heads of 256 each as two halves) and looks after key n's scales.
+  // Pages are asked for one stage ahead of the copies, and looked at only then.
+  const int shift = a.page_shift, in_page = a.page_tokens - 1, box_keys = min(a.page_tokens, KEYS);
+  constexpr int WIDE = HD / Tile::kBoxBytes;   // boxes a row is cut into
+  const int per_plane = KEYS / box_keys, boxes = 2 * per_plane * WIDE;
+  const int plane = lane / (per_plane * WIDE), box = lane % (per_plane * WIDE) / WIDE, wide = lane % WIDE;
+  auto page_of = [&](int i, int key) {   // the page of key `key` of stage i, as the table has it
+    const int slot = (first_of(i) + key) >> shift;
     return i < stages && slot < a.max_pages ? table[slot] : -1;
   };
   const int value_rows = a.kv_heads * a.page_tokens;   // from a key's row to its value's
-  const uint8_t* k_lane = a.codes + g * HD + t * 16;
-  const uint8_t* v_lane = a.codes + (static_cast<size_t>(value_rows) + 2 * t) * HD + g * Tile::kValueBytes;
-  auto copies = [&](int i, int key0, int page, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;   // every key of the stage is seen
-    unsigned char* at = ring + (i % STAGES) * Tile::kStageBytes;
-    const int key8 = key0 + lane % EIGHTS * 8;
-    bool there = page >= 0 && page < a.num_pages;
-    if (!there && key8 <= pos && (key8 + 8 > first_key || key8 < a.keep)) atomicOr(a.status, kStatusBadPage);
-    const int base = there ? (page * 2 * a.kv_heads + kv) * a.page_tokens + (key8 & in_page) : -1;   // the pool row of the eight's first key
-    auto seen = [&](int key) { return WHOLE || key_seen(key, pos, first_key, a.keep); };
-#pragma unroll
-    for (int b = 0; b < EIGHTS; ++b) {
-      const int from = __shfl_sync(0xffffffffu, base, b);
-      const size_t offset = static_cast<size_t>(max(from, 0)) * HD;
-      const bool k_there = from >= 0 && seen(key0 + b * 8 + g);
-#pragma unroll
-      for (int j = 0; j < Tile::kKeyPieces; ++j)
-        quant_copy<16>(at + ((b * Tile::kKeyPieces + j) * 32 + lane) * 16, k_lane + offset + j * 64, k_there);
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const bool v_there = from >= 0 && seen(key0 + b * 8 + 2 * t + n);
-#pragma unroll
-        for (int j = 0; j < Tile::kValuePieces; ++j)
-          quant_copy<Tile::kValueBytes>(at + Tile::kRowBytes + (((b * 2 + n) * Tile::kValuePieces + j) * 32 + lane) * Tile::kValueBytes,
-                                        v_lane + offset + n * HD + j * 128, v_there);
+  auto row_in = [&](int page, int key) { return (page * 2 * a.kv_heads + kv) * a.page_tokens + (key & in_page); };
+  // Every box of a stage is fetched: one that holds nothing the token sees starts behind the pool's last row, where the
+  // copy engine finds zeros.
+  auto issue = [&](int i, int box_page, int scale_page) {
+    if (i < stages) {
+      const int slot = i % STAGES, key0 = first_of(i);
+      if (lane == 0) barrier_arrive_expect(&landed[slot], 2 * Tile::kRowBytes);
+      __syncwarp();
+      if (lane < boxes) {
+        const int key = key0 + box * box_keys;
+        bool there = wanted(key, box_keys);
+        if (there && (box_page < 0 || box_page >= a.num_pages)) {
+          atomicOr(a.status, kStatusBadPage);
+          there = false;
+        }
+        tma_load_2d(ring + slot * (2 * Tile::kRowBytes) + plane * Tile::kRowBytes + wide * (KEYS * 128) + box * box_keys * Tile::kBoxBytes,
+                    &map_codes, wide * Tile::kBoxBytes,
+                    there ? row_in(box_page, key) + plane * value_rows : a.num_pages * 2 * value_rows, &landed[slot]);
       }
-    }
-    // a lane a key for the scales (heads of 256: lanes 16 to 31 the values')
-    const int key = lane % KEYS, from = __shfl_sync(0xffffffffu, base, key >> 3);
-    there = from >= 0 && seen(key0 + key);
-    const float* scale = a.scales + max(from, 0) + (key & 7);
-    at += 2 * Tile::kRowBytes;
-    if (KEYS == 32) {
-      quant_copy<4>(at + lane * 4, scale, there);
-      quant_copy<4>(at + (32 + lane) * 4, scale + value_rows, there);
-    } else {
-      quant_copy<4>(at + lane * 4, scale + (lane < KEYS ? 0 : value_rows), there);
-    }
-  };
-  auto issue = [&](int i, int page) {
-    const int key0 = first_of(i);
-    if (i < stages && holds(key0)) {
-      if (key0 >= first_key && key0 + KEYS - 1 <= pos) copies(i, key0, page, std::true_type());
-      else copies(i, key0, page, std::false_type());
+      const int key = key0 + lane % KEYS;
+      const bool there = key_seen(key, pos, first_key, a.keep) && scale_page >= 0 && scale_page < a.num_pages;
+      const float* scale = a.scales + (there ? row_in(scale_page, key) : 0);
+      float* to = ring_scales + slot * Tile::kScales + lane;
+      if (KEYS == 32) {
+        quant_copy_scale(to, scale, there);
+        quant_copy_scale(to + KEYS, scale + value_rows, there);
+      } else {
+        quant_copy_scale(to, scale + (lane < KEYS ? 0 : value_rows), there);
+      }
     }
     asm volatile("cp.async.commit_group;\n" ::);
   };
   // The token's own row, of the walk's last tile, is written by the kernel ahead of this one; with `settled` all others
   // are older, and their copies start ahead of the wait.
   bool waited = !a.settled;
-  int page = page_of(0);
+  const int box_key = box * box_keys, scale_key = lane % KEYS;
+  int box_page = page_of(0, box_key), scale_page = page_of(0, scale_key);
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) {
     if (!waited && i < stages && first_of(i) + KEYS > pos) {
       chain_wait();
       waited = true;
     }
-    const int next_page = page_of(i + 1);
-    issue(i, page);
-    page = next_page;
+    const int next_box = page_of(i + 1, box_key), next_scale = page_of(i + 1, scale_key);
+    issue(i, box_page, scale_page);
+    box_page = next_box;
+    scale_page = next_scale;
   }
   if (!waited) chain_wait();
 
   // ---- the query heads as rows 0..7 (float32: their second halves as rows 8..15)
+  auto key_chunk = [&](int j) { return HD == 64 ? t : (j >> 1) * 8 + 2 * t + (j & 1); };   // the lane's j-th chunk of a key row
   const bool scaled = BIASED || a.softcap > 0.0f;   // scores in natural units first; else in powers of two at once
   uint32_t q0[STEPS][PARTS], q2[STEPS][PARTS];
   float score_scale;
@@ -328,7 +363,7 @@ quantized_decode_mma_kernel(const QuantizedDecode a) {
     uint32_t largest = 0;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const T* at = q + (s >> 2) * 64 + t * 16 + (s & 3) * 4;
+      const T* at = q + key_chunk(s >> 2) * 16 + (s & 3) * 4;
       if (PARTS == 1) *reinterpret_cast<uint2*>(values[s]) = *reinterpret_cast<const uint2*>(at);
       else *reinterpret_cast<uint4*>(values[s]) = *reinterpret_cast<const uint4*>(at);
 #pragma unroll
@@ -346,51 +381,65 @@ quantized_decode_mma_kernel(const QuantizedDecode a) {
       split_pair<PARTS>(to_float(values[s][2]) * power, to_float(values[s][3]) * power, q2[s]);
     }
   }
-  float m_run = -INFINITY, l_run = 0.0f;   // of head g, over this warp's keys so far; the sum over this lane's alone
-  float top = 0.0f;
-  int ref = -100;                          // exponent of the reference, 2^floor(log2 top) but not below 2^-100
+  // From here on this lane deals with the heads 2t and 2t + 1 (columns of the products), with the keys g of every eight.
+  const float to_score[2] = {__shfl_sync(0xffffffffu, score_scale, 8 * t), __shfl_sync(0xffffffffu, score_scale, 8 * t + 4)};
+  float m[2] = {kQuantLow, kQuantLow}, l[2] = {0.0f, 0.0f};   // the reference, and this lane's share of the sum
+  float top[2] = {0.0f, 0.0f}, up[2] = {1.0f, 1.0f};
   float o[HD / 16][4];
 #pragma unroll
   for (int i = 0; i < HD / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  int given_up_at = stages;
 
   for (int i = 0; i < stages; ++i) {
+    const int slot = i % STAGES;
     asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2));
-    __syncwarp();   // every lane's copies of stage i have landed, and every lane is done with stage i - 1
-    const int next_page = page_of(i + STAGES);
-    issue(i + STAGES - 1, page);
-    page = next_page;
+    // Also where every lane's scales of stage i have landed, and every lane is done with stage i - 1. A wait that ran out
+    // says so in the status word; what is under way is waited for behind the loop.
+    if (!barrier_wait_warp(&landed[slot], (i / STAGES) & 1, a.status)) {
+      given_up_at = i;
+      break;
+    }
+    __syncwarp();
+    const int next_box = page_of(i + STAGES, box_key), next_scale = page_of(i + STAGES, scale_key);
+    issue(i + STAGES - 1, box_page, scale_page);
+    box_page = next_box;
+    scale_page = next_scale;
     const int key0 = first_of(i);
     if (!holds(key0)) continue;
-    const unsigned char* at = ring + (i % STAGES) * Tile::kStageBytes;
-    const float* scales = reinterpret_cast<const float*>(at + 2 * Tile::kRowBytes);
+    unsigned char* at = ring + slot * (2 * Tile::kRowBytes);
+    const float* scales = ring_scales + slot * Tile::kScales;
 
-    // ---- scores: this lane has those of head g and keys b * 8 + 2t, 2t + 1
+    // ---- scores: eight b, this lane has key b * 8 + g and heads 2t, 2t + 1
     float s[EIGHTS][2];
-    float d[EIGHTS][4];
+    {
+      float d[EIGHTS / 2][4];
 #pragma unroll
-    for (int b = 0; b < EIGHTS; ++b) d[b][0] = d[b][1] = d[b][2] = d[b][3] = 0.0f;
+      for (int h = 0; h < EIGHTS / 2; ++h) d[h][0] = d[h][1] = d[h][2] = d[h][3] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < Tile::kKeyPieces; ++j) {
-      uint32_t words[EIGHTS][4];
+      for (int j = 0; j < Tile::kChunks; ++j) {
+        uint32_t words[EIGHTS][4];
 #pragma unroll
-      for (int b = 0; b < EIGHTS; ++b)
-        *reinterpret_cast<uint4*>(words[b]) = *reinterpret_cast<const uint4*>(at + ((b * Tile::kKeyPieces + j) * 32 + lane) * 16);
+        for (int b = 0; b < EIGHTS; ++b)
+          *reinterpret_cast<uint4*>(words[b]) = *reinterpret_cast<const uint4*>(at + Tile::at(b * 8 + g, key_chunk(j)));
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int n = j * 4 + w;
+        for (int w = 0; w < 4; ++w) {
+          const int n = j * 4 + w;
 #pragma unroll
-        for (int b = 0; b < EIGHTS; ++b) {   // the eights' sums do not wait for one another
-          uint32_t b0, b1;
-          code_halves<KIND>(words[b][w], b0, b1);
-          quant_mma(d[b], q0[n][0], PARTS == 2 ? q0[n][PARTS - 1] : 0u, q2[n][0], PARTS == 2 ? q2[n][PARTS - 1] : 0u, b0, b1);
+          for (int h = 0; h < EIGHTS / 2; ++h) {
+            uint32_t a0, a1, a2, a3;
+            code_halves<KIND>(words[2 * h][w], a0, a2);
+            code_halves<KIND>(words[2 * h + 1][w], a1, a3);
+#pragma unroll
+            for (int x = 0; x < PARTS; ++x) quant_mma(d[h], a0, a1, a2, a3, q0[n][x], q2[n][x]);
+          }
         }
       }
-    }
 #pragma unroll
-    for (int b = 0; b < EIGHTS; ++b) {
-      const float2 k_scale = *reinterpret_cast<const float2*>(scales + b * 8 + 2 * t);
-      s[b][0] = (PARTS == 2 ? d[b][0] + d[b][2] : d[b][0]) * score_scale * k_scale.x;
-      s[b][1] = (PARTS == 2 ? d[b][1] + d[b][3] : d[b][1]) * score_scale * k_scale.y;
+      for (int b = 0; b < EIGHTS; ++b) {
+        const float k_scale = scales[b * 8 + g];
+        s[b][0] = d[b / 2][2 * (b & 1)] * to_score[0] * k_scale;
+        s[b][1] = d[b / 2][2 * (b & 1) + 1] * to_score[1] * k_scale;
+      }
     }
     if (scaled) {
 #pragma unroll
@@ -398,54 +447,80 @@ quantized_decode_mma_kernel(const QuantizedDecode a) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           s[b][j] = capped_score(s[b][j], a.softcap);
-          if (BIASED && g < live) s[b][j] += bias_at(a.bias.row(head0 + g), pos - (key0 + b * 8 + 2 * t + j), a.bias.far);
+          if (BIASED && 2 * t + j < live) s[b][j] += bias_at(a.bias.row(head0 + 2 * t + j), pos - (key0 + b * 8 + g), a.bias.far);
           s[b][j] *= kLog2E;
         }
     }
     if (key0 + KEYS - 1 > pos || key0 < first_key) {   // not every key of the stage is seen
 #pragma unroll
       for (int b = 0; b < EIGHTS; ++b)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (!key_seen(key0 + b * 8 + 2 * t + j, pos, first_key, a.keep)) s[b][j] = -INFINITY;
+        if (!key_seen(key0 + b * 8 + g, pos, first_key, a.keep)) s[b][0] = s[b][1] = -INFINITY;
     }
-    float m_new = m_run;
+    float weight[EIGHTS][2];
+    float sum[2], widest[2];
+    auto weigh = [&]() {
+      sum[0] = sum[1] = widest[0] = widest[1] = 0.0f;
 #pragma unroll
-    for (int b = 0; b < EIGHTS; ++b) m_new = fmaxf(m_new, fmaxf(s[b][0], s[b][1]));
-    m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, 1));
-    m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, 2));
-    const float zero = m_new == -INFINITY ? 0.0f : m_new;
-    const float carry = quant_exp2<T>(m_run - zero);   // what earlier stages gathered, on the new maximum (0 if nothing yet)
-    float l_new = 0.0f, widest = 0.0f;
+      for (int b = 0; b < EIGHTS; ++b) {
+        const float v_scale = scales[KEYS + b * 8 + g];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float p = quant_exp2<T>(s[b][j] - m[j]);
+          sum[j] += p;
+          weight[b][j] = p * v_scale;
+          widest[j] = fmaxf(widest[j], weight[b][j]);
+        }
+      }
+    };
+    weigh();
+    const bool outgrown = fmaxf(sum[0], sum[1]) > 65536.0f || fmaxf(widest[0] * up[0], widest[1] * up[1]) >= 32768.0f;
+    if (__any_sync(0xffffffffu, outgrown)) {
+      float carry[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float most = m[j];
+#pragma unroll
+        for (int b = 0; b < EIGHTS; ++b) most = fmaxf(most, s[b][j]);
+#pragma unroll
+        for (int offset = 4; offset < 32; offset <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
+        carry[j] = quant_exp2<T>(m[j] - most);   // what was gathered so far, on the new reference
+        m[j] = most;
+      }
+      weigh();
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float most = widest[j];
+#pragma unroll
+        for (int offset = 4; offset < 32; offset <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
+        top[j] = fmaxf(top[j] * carry[j], most);
+        const float before = up[j];
+        up[j] = power_of_two(kQuantTop - max(static_cast<int>(__float_as_uint(top[j]) >> 23) - 127, -100));
+        // a quotient beyond float32 means that what was gathered is nothing on the new reference: carry is 0 then
+        const float factor = carry[j] * fminf(up[j] / before, 0x1p127f);
+        l[j] *= carry[j];
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n) { o[n][j] *= factor; o[n][2 + j] *= factor; }
+      }
+    }
+    l[0] += sum[0];
+    l[1] += sum[1];
+    uint32_t p[EIGHTS][PARTS];   // keys b * 8 + 2t, 2t + 1 of head g
 #pragma unroll
     for (int b = 0; b < EIGHTS; ++b) {
-      const float p0 = quant_exp2<T>(s[b][0] - zero), p1 = quant_exp2<T>(s[b][1] - zero);
-      l_new += p0 + p1;
-      const float2 v_scale = *reinterpret_cast<const float2*>(scales + KEYS + b * 8 + 2 * t);
-      s[b][0] = p0 * v_scale.x;
-      s[b][1] = p1 * v_scale.y;
-      widest = fmaxf(widest, fmaxf(s[b][0], s[b][1]));
-    }
-    l_run = l_run * carry + l_new;
-    widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, 1));
-    widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, 2));
-    top = fmaxf(top * carry, widest);
-    const int ref_new = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);
-    const bool moved = m_new != m_run || ref_new != ref;
-    if (__any_sync(0xffffffffu, moved)) {
-      const float factor = moved ? carry * power_of_two(max(min(ref - ref_new, 127), -126)) : 1.0f;
-      const float c0 = __shfl_sync(0xffffffffu, factor, 8 * t), c1 = __shfl_sync(0xffffffffu, factor, 8 * t + 4);   // heads 2t, 2t + 1
+      split_pair<PARTS>(weight[b][0] * up[0], weight[b][1] * up[1], p[b]);
 #pragma unroll
-      for (int n = 0; n < HD / 16; ++n) { o[n][0] *= c0; o[n][1] *= c1; o[n][2] *= c0; o[n][3] *= c1; }
+      for (int x = 0; x < PARTS; ++x) p[b][x] = turn_tile(p[b][x]);
     }
-    m_run = m_new;
-    ref = ref_new;
-    const float up = power_of_two(14 - ref);
-    uint32_t p[EIGHTS][PARTS];   // the weights of key pairs b * 8 + 2t, 2t + 1, times the values' scales
-#pragma unroll
-    for (int b = 0; b < EIGHTS; ++b) split_pair<PARTS>(s[b][0] * up, s[b][1] * up, p[b]);
     // ---- o^T += V^T p^T, sixteen keys at a time
     at += Tile::kRowBytes;
+    if (key0 + KEYS - 1 > pos || key0 < first_key) {
+      // A key that is not seen has weight 0, but 0 x NaN is NaN: whatever its page's earlier owner left becomes zeros.
+      const int r = lane % KEYS, key = key0 + r;
+      if (!key_seen(key, pos, first_key, a.keep))
+        for (int c = lane / KEYS; c < HD / 16; c += 32 / KEYS) *reinterpret_cast<uint4*>(at + Tile::at(r, c)) = make_uint4(0u, 0u, 0u, 0u);
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // ahead of the copy that fills the slot next
+      __syncwarp();
+    }
 #pragma unroll
     for (int h = 0; h < KEYS / 16; ++h) {
 #pragma unroll
@@ -454,7 +529,8 @@ quantized_decode_mma_kernel(const QuantizedDecode a) {
         uint32_t v[4][WORDS];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const unsigned char* src = at + (((h * 4 + n) * Tile::kValuePieces + j) * 32 + lane) * Tile::kValueBytes;
+          const int r = h * 16 + 2 * t + (n & 1) + (n >> 1) * 8;
+          const unsigned char* src = at + (HD == 64 ? Tile::at(r, g >> 1) + (g & 1) * 8 : Tile::at(r, j * 8 + g));
           if (WORDS == 4) *reinterpret_cast<uint4*>(v[n]) = *reinterpret_cast<const uint4*>(src);
           else *reinterpret_cast<uint2*>(v[n]) = *reinterpret_cast<const uint2*>(src);
         }
@@ -474,15 +550,20 @@ quantized_decode_mma_kernel(const QuantizedDecode a) {
     }
   }
   asm volatile("cp.async.wait_group 0;\n" ::);
-  l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-  l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+  for (int i = given_up_at; i < stages && i < given_up_at + STAGES - 1; ++i)   // a warp that gives up waits for its copies under way
+    barrier_wait_warp(&landed[i % STAGES], (i / STAGES) & 1, a.status);
+#pragma unroll
+  for (int offset = 4; offset < 32; offset <<= 1) {
+    l[0] += __shfl_xor_sync(0xffffffffu, l[0], offset);
+    l[1] += __shfl_xor_sync(0xffffffffu, l[1], offset);
+  }
   if (release_late) chain_release();
 
   // ---- the four warps in warp order: this block's partial result (the area lies over the ring, which is used up)
   __syncthreads();
   float* merge = reinterpret_cast<float*>(quant_shared);   // [warps][8 heads][HD + 2]
   {
-    const float down = power_of_two(ref - 14), d0 = __shfl_sync(0xffffffffu, down, 8 * t), d1 = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+    const float d0 = 1.0f / up[0], d1 = 1.0f / up[1];   // powers of two
 #pragma unroll
     for (int n = 0; n < HD / 16; ++n) {
       constexpr int BLOCKS = Tile::kValueBytes / 2;   // of 16 values, from one piece
@@ -492,21 +573,24 @@ quantized_decode_mma_kernel(const QuantizedDecode a) {
       *reinterpret_cast<float2*>(to + HD + 2) = make_float2(o[n][1] * d1, o[n][3] * d1);
     }
   }
-  if (t == 0) {
-    merge[(warp * 8 + g) * (HD + 2) + HD] = m_run;
-    merge[(warp * 8 + g) * (HD + 2) + HD + 1] = l_run;
+  if (g == 0) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      merge[(warp * 8 + 2 * t + j) * (HD + 2) + HD] = m[j];
+      merge[(warp * 8 + 2 * t + j) * (HD + 2) + HD + 1] = l[j];
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < live * HD; i += kDecodeThreads) {
     const int h = i / HD, d = i - h * HD;
-    float m_all = -INFINITY;
+    float m_all = kQuantLow;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) m_all = fmaxf(m_all, merge[(w * 8 + h) * (HD + 2) + HD]);
     float sum = 0.0f, l_all = 0.0f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float* theirs = merge + (w * 8 + h) * (HD + 2);
-      const float weight = quant_exp2<T>(theirs[HD] - m_all);   // a warp without keys has m = -inf: weight 0
+      const float weight = quant_exp2<T>(theirs[HD] - m_all);   // a warp without keys has l = 0 and zeros
       sum += weight * theirs[d];
       l_all += weight * theirs[HD + 1];
     }
@@ -538,7 +622,12 @@ static cudaError_t launch_quantized_mma(const QuantizedDecode& args, dim3 grid, 
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, QuantTile<HD>::kShared);
     if (e != cudaSuccess) return e;
   }
-  return launch_chained(kernel, grid, dim3(kDecodeThreads), QuantTile<HD>::kShared, stream, args);
+  CUtensorMap map;
+  const int keys = QuantTile<HD>::kKeys;
+  if (!encode_codes_map(&map, args.codes, static_cast<long long>(args.num_pages) * 2 * args.kv_heads * args.page_tokens, HD,
+                        args.page_tokens < keys ? args.page_tokens : keys))
+    return cudaErrorInvalidValue;
+  return launch_chained(kernel, grid, dim3(kDecodeThreads), QuantTile<HD>::kShared, stream, map, args);
 }
 
 // Launches the kernel that takes the shape; `slots` says into how many partial results a pair was cut.
