@@ -4,9 +4,11 @@
 //
 // Work is cut as the kernels over a cache in the compute type cut it: a pair of
 // (token, key/value head) gets `slots` blocks, block s takes the tiles of
-// kSplitKeys keys first + s, first + s + slots, ... of the token's keys and leaves
-// one unnormalised partial result (accumulator, maximum, sum), which the merge
-// kernel puts together in slot order.
+// kSplitKeys keys first + s, first + s + slots, ... of the token's keys and ends with
+// one unnormalised partial result (accumulator, maximum, sum). Those of a pair are
+// put together in slot order, by the merge kernel or, where a pair's blocks are
+// few enough to be one cluster, by the blocks themselves out of one another's
+// shared memory.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -29,6 +31,14 @@ struct QuantizedDecode {
   int page_shift;                // log2 of page_tokens, -1 where that is no power of two
   int settled;                   // the positions ahead of each token's own were written by launches before the last one
   int* status;
+  // What the blocks of a cluster write where they put their results together themselves (`fused`: the slots of a pair are one cluster).
+  int fused, max_splits;
+  void* out;                     // [tokens, heads, head_dim]
+  const void* gate;              // optional, rows gate_stride values apart
+  long long gate_stride;
+  int has_sink;
+  float sink_score;
+  const float* sink_heads;
 };
 
 constexpr int kQuantHeads = 8;   // query heads of a block of the general kernel
@@ -171,7 +181,7 @@ template <int HD> struct QuantTile {
   static constexpr int kWarpBytes = kStages * 2 * kRowBytes;   // the ring's codes; its scales lie behind all warps' codes
   static constexpr int kScales = 2 * kKeys;                    // of a stage: keys', values'
   static constexpr int kRing = (kDecodeThreads / 32) * (kWarpBytes + kStages * kScales * 4);
-  static constexpr int kMerge = (kDecodeThreads / 32) * 8 * (HD + 2) * 4;
+  static constexpr int kMerge = (kDecodeThreads / 32 + 1) * 8 * (HD + 2) * 4;   // the warps' results and the block's
   static constexpr int kShared = (kRing > kMerge ? kRing : kMerge) + 1024;   // and room to align to the swizzle's period
   // Where chunk c of row r of a stage lies: the hardware's swizzle of 128-byte rows (64-byte ones for heads of 64).
   static __device__ __forceinline__ int at(int r, int c) {
@@ -246,6 +256,18 @@ __device__ __forceinline__ float power_of_two(int exponent) { return __uint_as_f
 
 template <typename T> __device__ __forceinline__ float quant_exp2(float x) { return std::is_same<T, float>::value ? exp2f(x) : decode_exp2(x); }
 
+__device__ __forceinline__ void quant_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
+// What lies at `mine` in the shared memory of the cluster's block `rank`.
+__device__ __forceinline__ float quant_peer(const float* mine, int rank) {
+  uint32_t address;
+  float value;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(address) : "r"(shared_address(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(value) : "r"(address) : "memory");
+  return value;
+}
+
 // Blocks resident on an SM: what the ring and the registers leave room for.
 template <typename T, int HD> struct QuantBlocks {
   static constexpr int value = HD == 256 ? (std::is_same<T, float>::value ? 1 : 2) : 3;
@@ -273,7 +295,43 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
   const int live = min(group - part * 8, 8), head0 = kv * group + part * 8;   // this block's query heads
   const int first_key = first_visible_key(pos, a.window, a.chunk);
   const KeyWalk walk = key_walk(first_key, pos, a.keep, kSplitKeys);
-  if (rank >= walk.count) return;   // more slots than tiles: the merge skips this one
+  if (pos / kSplitKeys >= a.max_splits) {   // beyond the caller's bound on the contexts: the row is left as it is
+    if (a.fused && rank == 0 && threadIdx.x == 0) atomicOr(a.status, kStatusBadSlot);
+    return;
+  }
+  // The end of a pair whose blocks are a cluster: every block's partial result lies at `results` in its shared memory,
+  // [8 heads][HD + 2] with maxima in powers of two, and a block writes every slots-th part of the output.
+  float* results = reinterpret_cast<float*>(quant_shared) + WARPS * 8 * (HD + 2);
+  auto finish = [&]() {
+    quant_cluster_sync();
+    const int parts_in = min(slots, walk.count);   // the others have nothing
+    for (int i = rank * kDecodeThreads + threadIdx.x; i < live * HD; i += slots * kDecodeThreads) {
+      const int h = i / HD, d = i - h * HD;
+      float m_all = kQuantLow, sum = 0.0f, l_all = 0.0f;
+      for (int b = 0; b < parts_in; ++b) m_all = fmaxf(m_all, quant_peer(results + h * (HD + 2) + HD, b));
+      for (int b = 0; b < parts_in; ++b) {
+        const float weight = quant_exp2<T>(quant_peer(results + h * (HD + 2) + HD, b) - m_all);
+        sum = fmaf(weight, quant_peer(results + h * (HD + 2) + d, b), sum);
+        l_all = fmaf(weight, quant_peer(results + h * (HD + 2) + HD + 1, b), l_all);
+      }
+      const int head = head0 + h;
+      if (a.has_sink) l_all += quant_exp2<T>((a.sink_heads != nullptr ? a.sink_heads[head] : a.sink_score) * kLog2E - m_all);
+      float value = sum / l_all;
+      if (a.gate != nullptr) {
+        const T* gate = behind_wait(static_cast<const T*>(a.gate)) + token * a.gate_stride;
+        value *= sigmoid_of(to_float(gate[static_cast<long long>(head) * HD + d]));
+      }
+      static_cast<T*>(a.out)[(static_cast<size_t>(token) * a.heads + head) * HD + d] = from_float<T>(value);
+    }
+    quant_cluster_sync();   // nobody leaves while its results are being read
+  };
+  if (rank >= walk.count) {   // more slots than tiles
+    if (a.fused) {
+      chain_wait();
+      finish();
+    }
+    return;
+  }
   const int* table = a.block_tables + static_cast<size_t>(a.row_request[row]) * a.max_pages;
   unsigned char* ring = quant_shared + warp * Tile::kWarpBytes;
   float* ring_scales = reinterpret_cast<float*>(quant_shared + WARPS * Tile::kWarpBytes) + warp * (STAGES * Tile::kScales);
@@ -594,10 +652,11 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
       sum += weight * theirs[d];
       l_all += weight * theirs[HD + 1];
     }
-    float* dst = a.partial + ((static_cast<size_t>(row) * a.heads + head0 + h) * slots + rank) * (HD + 2);
+    float* dst = a.fused ? results + h * (HD + 2) : a.partial + ((static_cast<size_t>(row) * a.heads + head0 + h) * slots + rank) * (HD + 2);
     dst[d] = sum;
-    if (d == 0) { dst[HD] = m_all * 0.6931471805599453f; dst[HD + 1] = l_all; }   // the merge kernel works in natural units
+    if (d == 0) { dst[HD] = a.fused ? m_all : m_all * 0.6931471805599453f; dst[HD + 1] = l_all; }   // the merge kernel works in natural units
   }
+  if (a.fused) finish();
 }
 
 // Whether the tensor-core kernel takes these rows: pieces of 16 bytes (queries: 8 or 16) that lie on such boundaries, and
@@ -607,12 +666,17 @@ static bool quantized_mma_takes(const QuantizedDecode& a) {
          reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
 }
 
-// How many blocks a (token, key/value head) pair gets: as many as fill the GPU
-// with blocks resident at once, no more than it has tiles.
-static int quantized_slots(int pairs, int max_splits, int resident) {
-  int wanted = pairs > 0 ? resident / pairs : 1;
-  if (wanted < 1) wanted = 1;
-  return wanted < max_splits ? wanted : max_splits;
+// How many blocks a (token, key/value head) pair gets of the tensor-core kernel, `tiles` being the most that one has and
+// `resident` how many blocks the GPU holds. Where that leaves blocks eight tiles or more, two rounds of blocks: the contexts of
+// a batch differ, and blocks of the longest would be alone for half the time (16 requests of up to 32,000 positions: 122 us
+// in one round, 92 in two; 8 of 32,000 each: 88 and 92). Else one round, and a tile or two a block where there are few.
+static int quantized_slots(int pairs, int tiles, int resident) {
+  const int twice = pairs <= resident ? 2 * resident / pairs : (2 * resident + pairs / 2) / pairs;
+  if (pairs > 1 && twice > 1 && tiles >= 8 * twice) return twice;
+  int slots = resident / pairs;
+  const int most = tiles <= 8 ? tiles : (tiles / 2 > 8 ? tiles / 2 : 8);
+  if (slots > most) slots = most;
+  return slots > 1 ? slots : 1;
 }
 
 template <typename T, int KIND, int HD>
@@ -627,23 +691,34 @@ static cudaError_t launch_quantized_mma(const QuantizedDecode& args, dim3 grid, 
   if (!encode_codes_map(&map, args.codes, static_cast<long long>(args.num_pages) * 2 * args.kv_heads * args.page_tokens, HD,
                         args.page_tokens < keys ? args.page_tokens : keys))
     return cudaErrorInvalidValue;
+  if (args.fused) return launch_chained_clusters(kernel, grid, dim3(kDecodeThreads), QuantTile<HD>::kShared, grid.x, stream, map, args);
   return launch_chained(kernel, grid, dim3(kDecodeThreads), QuantTile<HD>::kShared, stream, map, args);
 }
 
-// Launches the kernel that takes the shape; `slots` says into how many partial results a pair was cut.
+// Launches the kernel that takes the shape; `slots` says into how many partial results a pair was cut, 0 that the output
+// is made. `fusable`: the caller wants the output, not the partial results.
+constexpr int kQuantCluster = 8;   // blocks of a cluster, at most
 template <typename T>
-static cudaError_t launch_quantized_decode(const QuantizedDecode& args, int kind, int rows, int max_splits, int* slots, cudaStream_t stream) {
+static cudaError_t launch_quantized_decode(QuantizedDecode args, int kind, int rows, bool fusable, int* slots, cudaStream_t stream) {
   const int parts = (args.heads / args.kv_heads + kQuantHeads - 1) / kQuantHeads, pairs = rows * args.kv_heads * parts;
+  int tiles = args.max_splits;   // the most that a pair has
+  if (args.window > 0) tiles = min(tiles, (args.window + kSplitKeys - 1) / kSplitKeys + 1 + (args.keep + kSplitKeys - 1) / kSplitKeys);
+  if (args.chunk > 0) tiles = min(tiles, (args.chunk + kSplitKeys - 1) / kSplitKeys + 1 + (args.keep + kSplitKeys - 1) / kSplitKeys);
   if (quantized_mma_takes(args)) {
-    *slots = quantized_slots(pairs, max_splits, 148 * (args.head_dim == 256 ? QuantBlocks<T, 256>::value : QuantBlocks<T, 128>::value));
-    const dim3 grid(*slots, args.kv_heads * parts, rows);
+    int count = quantized_slots(pairs, tiles, 148 * (args.head_dim == 256 ? QuantBlocks<T, 256>::value : QuantBlocks<T, 128>::value));
+    // Few tiles over a few more blocks than a cluster has: the launch and the trip through memory that the merge kernel
+    // costs are worth more than the blocks.
+    if (fusable && count > kQuantCluster && tiles <= 6 * kQuantCluster) count = kQuantCluster;
+    args.fused = fusable && count <= kQuantCluster;
+    *slots = args.fused ? 0 : count;
+    const dim3 grid(count, args.kv_heads * parts, rows);
 #define BY_SIZE(KIND) (args.head_dim == 64    ? launch_quantized_mma<T, KIND, 64>(args, grid, stream)  \
                        : args.head_dim == 128 ? launch_quantized_mma<T, KIND, 128>(args, grid, stream) \
                                               : launch_quantized_mma<T, KIND, 256>(args, grid, stream))
     return kind == kCodesInt8 ? BY_SIZE(kCodesInt8) : BY_SIZE(kCodesE4M3);
 #undef BY_SIZE
   }
-  *slots = quantized_slots(pairs, max_splits, kDecodeBlocksAtOnce);
+  *slots = max(1, min(kDecodeBlocksAtOnce / static_cast<unsigned>(pairs), static_cast<unsigned>(args.max_splits)));
   const dim3 grid(*slots, args.kv_heads * parts, rows);
   auto launch = [&](auto kernel) {
     kernel<<<grid, kDecodeThreads, 0, stream>>>(args);
