@@ -1324,6 +1324,8 @@ struct QuantizedDecodeCall {
 // put together and projected by one kernel, as mxb_paged_attention_decode_project does.
 // settled: with chained launches on, the positions ahead of each token's own were
 // written by launches before the last one, and may be fetched while that one runs.
+// partial (float32, rows * heads * max_splits * (head_dim + 2) values) may be null:
+// where it is needed, cudaErrorNotReady says so and nothing has been launched.
 MXB_API int mxb_paged_attention_decode_quantized(const void* call, int bytes, cudaStream_t stream) {
   if (bytes != static_cast<int>(sizeof(QuantizedDecodeCall))) return static_cast<int>(cudaErrorInvalidValue);
   const QuantizedDecodeCall& c = *static_cast<const QuantizedDecodeCall*>(call);

@@ -260,6 +260,17 @@ def status_word(device) -> torch.Tensor:
     return word
 
 
+_status_pointers = {}
+
+
+def _status_pointer(index: int) -> int:
+    """The address of a device's status word (which stays where it is)."""
+    pointer = _status_pointers.get(index)
+    if pointer is None:
+        pointer = _status_pointers[index] = status_word(torch.device("cuda", index)).data_ptr()
+    return pointer
+
+
 _status_host = {}
 
 
@@ -1351,26 +1362,19 @@ class QuantizedPool:
         return _CODE_KINDS[self.codes.dtype]
 
 
-def _all_on(device: int, *tensors) -> bool:
-    """Whether all the tensors (those that are not None) are on CUDA device ``device``."""
-    for tensor in tensors:
-        if tensor is not None and tensor.get_device() != device:
-            return False
-    return True
-
-
 def _on_current_device(*tensors) -> None:
     """The kernels run on the current device's current stream: everything has to be there."""
     current = _current_device()
-    if not _all_on(current, *tensors):
-        raise KernelError(f"a tensor is on another device than the current one (cuda:{current})")
-
-
-def _int_lists(dims: int, *tensors) -> bool:
-    """Whether all are contiguous int32 tensors of so many dimensions."""
     for tensor in tensors:
-        if not (isinstance(tensor, torch.Tensor) and tensor.dtype is torch.int32 and tensor.dim() == dims
-                and tensor.is_contiguous() and tensor.is_cuda):
+        if tensor is not None and tensor.get_device() != current:
+            raise KernelError(f"a tensor is on another device than the current one (cuda:{current})")
+
+
+def _ints_on(device: int, dims: int, *tensors) -> bool:
+    """Whether all are contiguous int32 tensors of so many dimensions on CUDA device ``device``."""
+    for tensor in tensors:
+        if not (isinstance(tensor, torch.Tensor) and tensor.dtype is torch.int32 and tensor.get_device() == device
+                and tensor.dim() == dims and tensor.is_contiguous()):
             return False
     return True
 
@@ -1392,10 +1396,12 @@ def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tenso
     ``last`` reads nothing."""
     _need(isinstance(pool, QuantizedPool), "pool must be a QuantizedPool")
     codes = pool.codes
-    shape = codes.shape
+    shape, device = codes.shape, codes.get_device()
     rows = row_request.numel() if isinstance(row_request, torch.Tensor) else 0
-    if not (isinstance(out, torch.Tensor) and out.dtype in _CODES and out.shape == shape and out.is_contiguous() and _int_lists(2, block_tables)
-            and _int_lists(1, row_request, first, last) and first.numel() == last.numel() == rows <= 65535 and shape[4] <= 512):
+    if not (isinstance(out, torch.Tensor) and out.dtype in _CODES and out.shape == shape and out.is_contiguous()
+            and out.get_device() == device == _current_device() and _ints_on(device, 2, block_tables)
+            and _ints_on(device, 1, row_request, first, last) and first.numel() == last.numel() == rows <= 65535
+            and shape[4] <= 512):
         _check(out, "out", tuple(_CODES), 5)
         _need(out.shape == shape, "out must have the pool's shape")
         _check(block_tables, "block_tables", (torch.int32,), 2)
@@ -1404,13 +1410,14 @@ def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tenso
         _need(first.numel() == rows and last.numel() == rows, "row lists differ in length")
         _need(rows <= 65535, f"{rows} rows in one call; up to 65535")
         _need(shape[4] <= 512, f"head_dim {shape[4]} is beyond 512")
-    _on_current_device(codes, out, block_tables, row_request, first, last)
+        _on_current_device(codes, out, block_tables, row_request, first, last)
     if rows and codes.numel():
         num_pages, _, kv_heads, page_tokens, head_dim = shape
         call = _READ_CALL.pack(
             codes.data_ptr(), pool.scales.data_ptr(), out.data_ptr(), block_tables.data_ptr(), row_request.data_ptr(),
-            first.data_ptr(), last.data_ptr(), status_word(out.device).data_ptr(), _CODE_KINDS[codes.dtype], _CODES[out.dtype],
-            block_tables.shape[1], rows, kv_heads, head_dim, page_tokens, num_pages, window or 0, chunk or 0, _kept(keep))
+            first.data_ptr(), last.data_ptr(), _status_pointer(device), _CODE_KINDS[codes.dtype], _CODES[out.dtype],
+            block_tables.shape[1], rows, kv_heads, head_dim, page_tokens, num_pages, window or 0, chunk or 0,
+            _kept(keep) if keep else 0)
         _call("mxb_read_cache", call, len(call), _stream())
     return out
 
@@ -1433,6 +1440,10 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
     the rows, unrounded, as codes and scales). q, k and v are
     [tokens, heads * head_dim] views whose rows may be strided. ``q_factors``
     (float32, one per position): what the queries are multiplied by."""
+    if isinstance(cache, QuantizedPool):
+        _store_quantized(q, k, v, q_out, cache, slots, positions, q_weight, k_weight, cos, sin, eps, interleaved, norm_scope,
+                         q_factors)
+        return
     dtype = q.dtype
     for name, tensor in (("q", q), ("k", k), ("v", v)):
         _need(tensor.is_cuda and tensor.dtype == dtype and tensor.dtype in _CODES and tensor.dim() == 2
@@ -1440,10 +1451,8 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
     tokens = q.shape[0]
     _check(positions, "positions", (torch.int32,), 1)
     _need(positions.numel() == tokens and k.shape[0] == tokens and v.shape[0] == tokens, "token counts differ")
-    quantized = isinstance(cache, QuantizedPool)
     if cache is not None:
-        if not quantized:
-            _check(cache, "cache", (dtype,), 5)
+        _check(cache, "cache", (dtype,), 5)
         num_pages, two, kv_heads, page_tokens, head_dim = cache.shape
         _need(two == 2, "cache must be [pages, 2, kv_heads, page_tokens, head_dim]")
         _check(slots, "slots", (torch.int32,), 1)
@@ -1476,21 +1485,6 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
         _need(rotary_dim <= head_dim, "rotary_dim exceeds head_dim")
     if q_factors is not None:
         _check(q_factors, "q_factors", (torch.float32,), 1)
-    if quantized:
-        if head_dim > 512 or heads + 2 * kv_heads > 65535:
-            raise KernelError(f"{heads} + 2 x {kv_heads} heads of {head_dim} values")
-        _on_current_device(cache.codes, q, k, v, q_out, slots, positions, q_weight, k_weight, cos, sin, q_factors)
-        projection = norm_scope == "projection" and (q_weight is not None or k_weight is not None)
-        sums = torch.empty(2 * tokens, dtype=torch.float32, device=q.device) if projection else None
-        call = _STORE_CALL.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_out) or 0, cache.codes.data_ptr(), cache.scales.data_ptr(),
-            slots.data_ptr(), positions.data_ptr(), _ptr(q_weight) or 0, _ptr(k_weight) or 0, _ptr(cos) or 0, _ptr(sin) or 0,
-            _ptr(sums) or 0, _ptr(q_factors) or 0, status_word(q.device).data_ptr(), q.stride(0), k.stride(0), v.stride(0),
-            _CODE_KINDS[cache.codes.dtype], _CODES[dtype], table_positions, rotary_dim, 1 if interleaved else 0,
-            1 if projection else 0, tokens, heads, kv_heads, head_dim, page_tokens, num_pages,
-            q_factors.numel() if q_factors is not None else 0, eps)
-        _call("mxb_store_quantized", call, len(call), _stream())
-        return
     _call("mxb_qk_norm_rope_cache", q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0),
           v.stride(0), _ptr(q_out), _ptr(cache), _ptr(slots), positions.data_ptr(), _ptr(q_weight),
           _ptr(k_weight), _ptr(cos), _ptr(sin), table_positions, rotary_dim, 1 if interleaved else 0,
@@ -1498,6 +1492,67 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
           head_dim, page_tokens, num_pages, float(eps), _CODES[dtype], _ptr(q_factors),
           q_factors.numel() if q_factors is not None else 0,
           status_word(q.device).data_ptr(), _stream())
+
+
+def _store_quantized(q, k, v, q_out, pool: QuantizedPool, slots, positions, q_weight, k_weight, cos, sin, eps: float,
+                     interleaved: bool, norm_scope: str, q_factors) -> None:
+    """``qk_norm_rope_cache`` into a quantized pool."""
+    codes, dtype = pool.codes, q.dtype
+    device = codes.get_device()
+    num_pages, _, kv_heads, page_tokens, head_dim = codes.shape
+    for tensor in (q, k, v):
+        if not (tensor.dtype is dtype and tensor.dim() == 2 and tensor.stride(1) == 1 and tensor.get_device() == device
+                and dtype in _CODES):
+            raise KernelError("q, k and v must be CUDA [tokens, width] tensors with unit column stride, of one type and on the "
+                              "pool's device")
+    tokens, width = q.shape
+    heads = width // head_dim
+    if not (width == heads * head_dim and k.shape == v.shape == (tokens, kv_heads * head_dim)):
+        _need(k.shape[0] == tokens and v.shape[0] == tokens, "token counts differ")
+        raise KernelError("q, k, v widths do not match the head layout")
+    if not (_ints_on(device, 1, slots, positions) and slots.numel() == positions.numel() == tokens and device == _current_device()):
+        _check(positions, "positions", (torch.int32,), 1)
+        _check(slots, "slots", (torch.int32,), 1)
+        _need(positions.numel() == tokens, "token counts differ")
+        _need(slots.numel() == tokens, "one slot per token")
+        _on_current_device(codes, slots, positions)
+    _need(head_dim <= 512 and heads + 2 * kv_heads <= 65535, "heads of up to 512 values, up to 65535 of them")
+    if q_out is not None and not (q_out.dtype is dtype and q_out.is_contiguous() and q_out.shape == (tokens, heads, head_dim)
+                                  and q_out.get_device() == device):
+        _check(q_out, "q_out", (dtype,), 3)
+        _need(q_out.shape == (tokens, heads, head_dim), "q_out must be [tokens, heads, head_dim]")
+        _on_current_device(q_out)
+    _need(norm_scope == "head" or norm_scope == "projection", "unknown norm scope")
+    projection = norm_scope == "projection" and (q_weight is not None or k_weight is not None)
+    for weight, values in ((q_weight, heads * head_dim if projection else head_dim),
+                           (k_weight, kv_heads * head_dim if projection else head_dim)):
+        if weight is not None and not (weight.dtype is torch.float32 and weight.is_contiguous() and weight.dim() == 1
+                                       and weight.numel() == values and weight.get_device() == device):
+            _check(weight, "a norm's weight", (torch.float32,), 1)
+            _need(weight.numel() == values, f"a norm's weight has {weight.numel()} values, {values} are needed")
+            _on_current_device(weight)
+    rotary_dim = table_positions = factors = 0
+    if cos is not None:
+        if not (sin is not None and cos.dtype is sin.dtype is torch.float32 and cos.is_contiguous() and sin.is_contiguous()
+                and cos.dim() == 2 and cos.shape == sin.shape and cos.get_device() == sin.get_device() == device):
+            _check(cos, "cos", (torch.float32,), 2)
+            _check(sin, "sin", (torch.float32,), 2)
+            _need(cos.shape == sin.shape, "cos and sin differ in shape")
+            _on_current_device(cos, sin)
+        table_positions, rotary_dim = cos.shape[0], cos.shape[1] * 2
+        _need(rotary_dim <= head_dim, "rotary_dim exceeds head_dim")
+    if q_factors is not None:
+        _check(q_factors, "q_factors", (torch.float32,), 1)
+        _on_current_device(q_factors)
+        factors = q_factors.numel()
+    sums = torch.empty(2 * tokens, dtype=torch.float32, device=q.device) if projection else None
+    call = _STORE_CALL.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_out) or 0, codes.data_ptr(), pool.scales.data_ptr(),
+        slots.data_ptr(), positions.data_ptr(), _ptr(q_weight) or 0, _ptr(k_weight) or 0, _ptr(cos) or 0, _ptr(sin) or 0,
+        _ptr(sums) or 0, _ptr(q_factors) or 0, _status_pointer(device), q.stride(0), k.stride(0), v.stride(0),
+        _CODE_KINDS[codes.dtype], _CODES[dtype], table_positions, rotary_dim, 1 if interleaved else 0, 1 if projection else 0,
+        tokens, heads, kv_heads, head_dim, page_tokens, num_pages, factors, eps)
+    _call("mxb_store_quantized", call, len(call), _stream())
 
 
 def norm_rotate_heads(x: torch.Tensor, head_dim: int, positions: torch.Tensor,
@@ -1762,11 +1817,19 @@ def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.
     output projection ``weight``, into ``summands``."""
     global _split_keys
     codes, dtype = pool.codes, q.dtype
+    device = codes.get_device()
     num_pages, _, kv_heads, page_tokens, cache_dim = codes.shape
+    if not (q.dim() == 3 and dtype in _CODES and q.is_contiguous() and q.get_device() == device == _current_device()
+            and (out is None or (out.dtype is dtype and out.shape == q.shape and out.is_contiguous() and out.get_device() == device))):
+        _check(q, "q", _COMPUTE, 3)
+        if out is not None:
+            _check(out, "out", (dtype,), 3)
+            _need(out.shape == q.shape, "out and q differ in shape")
+        _on_current_device(codes, q, out)
     tokens, heads, head_dim = q.shape
     rows = row_token.numel()
-    if not (cache_dim == head_dim and quantized_decode_supported(head_dim, heads, kv_heads, dtype) and softcap >= 0.0
-            and _int_lists(2, block_tables) and _int_lists(1, row_token, row_request, positions)
+    if not (cache_dim == head_dim <= 256 and head_dim and heads >= kv_heads and heads % kv_heads == 0 and softcap >= 0.0
+            and _ints_on(device, 2, block_tables) and _ints_on(device, 1, row_token, row_request, positions)
             and row_request.numel() == rows <= 65535 and positions.numel() == tokens):
         _need(softcap >= 0.0, "the cap on the scores cannot be negative")
         _need(cache_dim == head_dim, f"the pool's rows are {cache_dim} values wide, the queries {head_dim}")
@@ -1777,32 +1840,48 @@ def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.
             _check(tensor, name, (torch.int32,), 1)
         _need(row_request.numel() == rows and positions.numel() == tokens, "row lists do not fit")
         _need(rows <= 65535, f"{rows} rows in one call; up to 65535")
+        _on_current_device(block_tables, row_token, row_request, positions)
     if _split_keys is None:
         _split_keys = decode_split_keys()
     splits = max(1, -(-int(longest_context) // _split_keys))
     need = rows * heads * splits * (head_dim + 2)
-    if partial is None:
-        partial = torch.empty(need, dtype=torch.float32, device=q.device)
-    elif not (partial.dtype is torch.float32 and partial.is_contiguous() and partial.numel() >= need):
+    if partial is not None and not (partial.dtype is torch.float32 and partial.is_contiguous() and partial.numel() >= need):
         _check(partial, "partial", (torch.float32,))
         _need(partial.numel() >= need, f"partial holds {partial.numel()} values, {need} are needed")
-    gate_stride = _gate_stride(gate, q)
-    has_sink, sink_score, sink_heads = _sink(sink, heads)
-    bias_table, bias_far = _score_bias(bias, heads)
-    _on_current_device(codes, q, out, block_tables, row_token, row_request, positions, partial, gate, weight,
-                       sink if sink_heads else None, bias)
-    hidden, ldw = (weight.shape[0], weight.stride(0)) if weight is not None else (0, 0)
+    gate_stride = hidden = ldw = has_sink = bias_far = 0
+    sink_score, sink_heads, bias_table = 0.0, None, None
+    if gate is not None:
+        gate_stride = _gate_stride(gate, q)
+    if sink is not None:
+        has_sink, sink_score, sink_heads = _sink(sink, heads)
+    if bias is not None:
+        bias_table, bias_far = _score_bias(bias, heads)
+    if weight is not None:
+        hidden, ldw = weight.shape[0], weight.stride(0)
+    if gate is not None or weight is not None or partial is not None or sink_heads or bias is not None:
+        _on_current_device(partial, gate, weight, sink if sink_heads else None, bias)
     if not rows:
         return
-    call = _QUANTIZED_DECODE_CALL.pack(
-        q.data_ptr(), codes.data_ptr(), pool.scales.data_ptr(), _ptr(out) or 0, partial.data_ptr(), block_tables.data_ptr(),
+    fields = [
+        q.data_ptr(), codes.data_ptr(), pool.scales.data_ptr(), _ptr(out) or 0, _ptr(partial) or 0, block_tables.data_ptr(),
         row_token.data_ptr(), row_request.data_ptr(), positions.data_ptr(), _ptr(weight) or 0, _ptr(summands) or 0, _ptr(gate) or 0,
-        sink_heads or 0, bias_table or 0, status_word(q.device).data_ptr(), _CODE_KINDS[codes.dtype], _CODES[dtype],
+        sink_heads or 0, bias_table or 0, _status_pointer(device), _CODE_KINDS[codes.dtype], _CODES[dtype],
         block_tables.shape[1], rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits, window or 0, chunk or 0,
-        _kept(keep), ldw, hidden, gate_stride, has_sink, bias_far, 1 if settled else 0, scale, softcap, sink_score)
-    _call("mxb_paged_attention_decode_quantized", call, len(call), _stream())
+        _kept(keep) if keep else 0, ldw, hidden, gate_stride, has_sink, bias_far, 1 if settled else 0, scale, softcap, sink_score]
+    call, stream = _QUANTIZED_DECODE_CALL.pack(*fields), _stream()
+    entry = _fn("mxb_paged_attention_decode_quantized")
+    code = entry(call, len(call), stream)
+    if code == _NOT_READY and partial is None:   # a pair's blocks are too many to put their results together themselves
+        partial = torch.empty(need, dtype=torch.float32, device=q.device)
+        fields[4] = partial.data_ptr()
+        call = _QUANTIZED_DECODE_CALL.pack(*fields)
+        code = entry(call, len(call), stream)
+    if code != 0:
+        raise KernelError(f"mxb_paged_attention_decode_quantized failed to launch: CUDA error {code}")
+    count_launches(1)
 
 
+_NOT_READY = 600   # cudaErrorNotReady
 _split_keys: Optional[int] = None
 
 
@@ -1831,18 +1910,17 @@ def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
     of each token's own were written by launches before the last one, so that
     with chained launches on they may be fetched while that one runs (a cache in
     the compute type is taken to be so)."""
-    dtype = q.dtype
-    if not softcap >= 0.0:
-        raise KernelError("the cap on the scores cannot be negative")
-    _check(q, "q", _COMPUTE, 3)
-    _check(out, "out", (dtype,), 3)
-    if out.shape != q.shape:
-        raise KernelError("out and q differ in shape")
     if isinstance(cache, QuantizedPool):
+        _need(out is not None, "out must be a tensor")
         _decode_quantized(q, cache, out, block_tables, row_token, row_request, positions, scale, longest_context, window,
                           partial, chunk, gate, softcap, sink, bias, keep, settled, None, None)
         return out
+    dtype = q.dtype
+    _need(softcap >= 0.0, "the cap on the scores cannot be negative")
+    _check(q, "q", tuple(_CODES), 3)
+    _check(out, "out", (dtype,), 3)
     _check(cache, "cache", (dtype,), 5)
+    _need(out.shape == q.shape, "out and q differ in shape")
     tokens, heads, head_dim = q.shape
     num_pages, two, kv_heads, page_tokens, cache_dim = cache.shape
     _need(two == 2 and cache_dim == head_dim, "cache must be [pages, 2, kv_heads, page_tokens, head_dim]")
