@@ -11,8 +11,6 @@
 // shared memory.
 #pragma once
 
-#include <cuda_fp16.h>
-
 #include "quantized.cuh"
 
 namespace mxb {
@@ -206,23 +204,6 @@ static bool encode_codes_map(CUtensorMap* map, const void* codes, long long rows
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, boxes, element_strides,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// The four codes of a word as two pairs of halves. Whole numbers: with its sign
-// bit turned a code is an unsigned u = code + 128, and the half with the bits
-// 0x6400 + u is 1024 + u.
-template <int KIND> __device__ __forceinline__ void code_halves(uint32_t word, uint32_t& lower, uint32_t& upper) {
-  if (KIND == kCodesE4M3) {
-    asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\ncvt.rn.f16x2.e4m3x2 %0, lo;\ncvt.rn.f16x2.e4m3x2 %1, hi;\n}\n"
-        : "=r"(lower), "=r"(upper) : "r"(word));
-  } else {
-    const uint32_t turned = word ^ 0x80808080u, off = 0xe480e480u;   // -1152
-    const __half2 less = *reinterpret_cast<const __half2*>(&off);
-    const uint32_t lo = __byte_perm(turned, 0x64646464u, 0x4140), hi = __byte_perm(turned, 0x64646464u, 0x4342);
-    const __half2 a = __hadd2(*reinterpret_cast<const __half2*>(&lo), less), b = __hadd2(*reinterpret_cast<const __half2*>(&hi), less);
-    lower = *reinterpret_cast<const uint32_t*>(&a);
-    upper = *reinterpret_cast<const uint32_t*>(&b);
-  }
 }
 
 __device__ __forceinline__ void quant_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

@@ -13,6 +13,7 @@
 // scales [pages, 2, kv_heads, page_tokens].
 #pragma once
 
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -27,6 +28,23 @@ template <int KIND> struct CodeLimit { static constexpr float value = KIND == kC
 template <int KIND> __device__ __forceinline__ float code_value(uint32_t byte) {
   if (KIND == kCodesInt8) return static_cast<float>(static_cast<int8_t>(byte));
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+}
+
+// The four codes of a word as two pairs of halves. Whole numbers: with its sign
+// bit turned a code is an unsigned u = code + 128, and the half with the bits
+// 0x6400 + u is 1024 + u.
+template <int KIND> __device__ __forceinline__ void code_halves(uint32_t word, uint32_t& lower, uint32_t& upper) {
+  if (KIND == kCodesE4M3) {
+    asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\ncvt.rn.f16x2.e4m3x2 %0, lo;\ncvt.rn.f16x2.e4m3x2 %1, hi;\n}\n"
+        : "=r"(lower), "=r"(upper) : "r"(word));
+  } else {
+    const uint32_t turned = word ^ 0x80808080u, off = 0xe480e480u;   // -1152
+    const __half2 less = *reinterpret_cast<const __half2*>(&off);
+    const uint32_t lo = __byte_perm(turned, 0x64646464u, 0x4140), hi = __byte_perm(turned, 0x64646464u, 0x4342);
+    const __half2 a = __hadd2(*reinterpret_cast<const __half2*>(&lo), less), b = __hadd2(*reinterpret_cast<const __half2*>(&hi), less);
+    lower = *reinterpret_cast<const uint32_t*>(&a);
+    upper = *reinterpret_cast<const uint32_t*>(&b);
+  }
 }
 
 // What a row's codes are made with. `largest` holds the bits of max |x|: as
@@ -68,6 +86,28 @@ __device__ __forceinline__ float odd_quotient(float x, const RowScale& r) {
     y = __uint_as_float(bits | 1u);
   }
   return y;
+}
+
+// Four values' codes as the bytes of a word.
+template <int KIND> __device__ __forceinline__ uint32_t four_codes(const float* x, const RowScale& r) {
+  if (r.inverse == 0.0f) return 0u;   // a row of zeros, or one that is not finite
+  float y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = odd_quotient(x[j], r);
+  if (KIND == kCodesE4M3) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+  }
+  if (r.shift != 1.0f) {   // scales among the smallest numbers are coarse: their quotients may lie beyond 127.5
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = fminf(fmaxf(y[j], -127.0f), 127.0f);
+  }
+  // to the nearest even by the sum's own rounding: |y| is at most 127 and an ulp, and the low byte is the code's
+  uint32_t c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c[j] = __float_as_uint(__fadd_rn(y[j], 12582912.0f));   // 1.5 x 2^23
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
 template <int KIND> __device__ __forceinline__ uint32_t code_of(float x, const RowScale& r) {

@@ -147,15 +147,21 @@ __global__ void __launch_bounds__(256) store_quantized_kernel(const StoreArgs a)
 // lanes. Run A of lane s starts at 8 s and run B half the rotated values
 // further (rotations of halves), or they are neighbours (neighbouring pairs, and
 // the values behind the rotated ones); either way the lane needs the cosines
-// 8 s ... 8 s + 7. Bound by its loads and stores.
+// 8 s ... 8 s + 7. Issue slots and the wait for positions, cosines and rows bind
+// it, so warps of queries end at their rotation (2,048 tokens of 32 / 8 heads of
+// 128: 20.6 us when they took the codes' part too, 18.0; the write of the same
+// rows in bfloat16 takes 14.5). Two or four heads a lane with one set of weights
+// and cosines, as that write does it, lose more warps than they save loads
+// (20.5 and 22.4 us).
 template <typename T, int KIND, int HD>
-__global__ void __launch_bounds__(256) store_quantized_lanes_kernel(const StoreArgs a) {
+__global__ void __launch_bounds__(256) store_quantized_lanes_kernel(const __grid_constant__ StoreArgs a) {
   constexpr int LANES = HD / 16, HEADS = 32 / LANES;   // lanes of a head, heads of a warp
   constexpr int WORDS = 8 * sizeof(T) / 16;            // 16-byte words of a run
   chain_release();
   // Up to chain_wait(): only the step's integers and what no kernel of a step writes.
   const int lane = threadIdx.x & 31, sub = lane % LANES;
-  const unsigned per_token = a.heads + 2 * a.kv_heads, total = static_cast<unsigned>(a.tokens) * per_token;   // below 2^31: the launcher sees to it
+  const unsigned per_token = a.heads + 2 * a.kv_heads;
+  const unsigned total = static_cast<unsigned>(a.tokens) * per_token;   // below 2^31: the launcher sees to it
   const unsigned item = (blockIdx.x * 8u + (threadIdx.x >> 5)) * HEADS + lane / LANES;
   bool active = item < total;   // lanes without work stay to the end: the others exchange values with their warp
   const int t = active ? static_cast<int>(item / per_token) : 0;
@@ -187,10 +193,6 @@ __global__ void __launch_bounds__(256) store_quantized_lanes_kernel(const StoreA
   const int at_a = apart ? 8 * sub : 16 * sub, at_b = apart ? half + 8 * sub : 16 * sub + 8;
   const float* weight = is_q ? a.q_weight : (is_k ? a.k_weight : nullptr);
   float gain[16], c[8], sn[8];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) gain[j] = 1.0f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) { c[j] = 1.0f; sn[j] = 0.0f; }
   auto floats = [](float* to, const float* from) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -198,8 +200,9 @@ __global__ void __launch_bounds__(256) store_quantized_lanes_kernel(const StoreA
       to[4 * w] = x.x; to[4 * w + 1] = x.y; to[4 * w + 2] = x.z; to[4 * w + 3] = x.w;
     }
   };
-  if (active && weight != nullptr) {
-    if (a.row_sums != nullptr) weight += static_cast<size_t>(is_q ? h : kv) * HD;
+  const bool normed = active && weight != nullptr;
+  if (normed) {
+    if (a.row_sums != nullptr) weight += static_cast<size_t>(is_q ? h : kv) * HD;   // a norm over the whole projection has weights for every head
     floats(gain, weight + at_a);
     floats(gain + 8, weight + at_b);
   }
@@ -230,23 +233,23 @@ __global__ void __launch_bounds__(256) store_quantized_lanes_kernel(const StoreA
       reinterpret_cast<uint4*>(in)[WORDS + w] = reinterpret_cast<const uint4*>(src + at_b)[w];
     }
   }
-  float x[16], sum = 0.0f;
+  float x[16];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    x[j] = to_float(in[j]);
-    sum += x[j] * x[j];
-  }
+  for (int j = 0; j < 16; ++j) x[j] = to_float(in[j]);
   if (a.q_weight != nullptr || a.k_weight != nullptr) {   // the same for the whole launch
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sum += x[j] * x[j];
 #pragma unroll
     for (int offset = LANES / 2; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-    if (weight != nullptr) {
+    if (normed) {
       const float mean = a.row_sums != nullptr ? behind_wait(a.row_sums)[2 * t + (is_k ? 1 : 0)] : sum / static_cast<float>(HD);
       const float scale = rsqrtf(mean + a.eps);
 #pragma unroll
       for (int j = 0; j < 16; ++j) x[j] = x[j] * scale * gain[j];
     }
   }
-  if (turns) {
+  if (turns && active) {
     if (a.interleaved) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -263,13 +266,7 @@ __global__ void __launch_bounds__(256) store_quantized_lanes_kernel(const StoreA
       }
     }
   }
-  uint32_t largest = 0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) largest = max(largest, magnitude_bits(x[j]));
-#pragma unroll
-  for (int offset = LANES / 2; offset > 0; offset >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
-  if (!active) return;
-  if (is_q) {
+  if (active && is_q) {
     alignas(16) T out[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) out[j] = from_float<T>(x[j] * factor);
@@ -279,27 +276,39 @@ __global__ void __launch_bounds__(256) store_quantized_lanes_kernel(const StoreA
       reinterpret_cast<uint4*>(dst + at_a)[w] = reinterpret_cast<const uint4*>(out)[w];
       reinterpret_cast<uint4*>(dst + at_b)[w] = reinterpret_cast<const uint4*>(out)[WORDS + w];
     }
-    return;
   }
-  const RowScale row = row_scale<KIND>(largest);
-  uint32_t words[4];
+  if (!__any_sync(0xffffffffu, active && !is_q)) return;   // a warp of queries
+  uint32_t largest = 0;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    words[w] = 0;
+  for (int j = 0; j < 16; ++j) largest = max(largest, magnitude_bits(x[j]));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) words[w] |= code_of<KIND>(x[4 * w + j], row) << (8 * j);
+  for (int offset = LANES / 2; offset > 0; offset >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
+  if (active && !is_q) {
+    const RowScale row = row_scale<KIND>(largest);
+    uint8_t* dst = a.codes + pool_row * HD;
+    *reinterpret_cast<uint2*>(dst + at_a) = make_uint2(four_codes<KIND>(x, row), four_codes<KIND>(x + 4, row));
+    *reinterpret_cast<uint2*>(dst + at_b) = make_uint2(four_codes<KIND>(x + 8, row), four_codes<KIND>(x + 12, row));
+    if (sub == 0) a.scales[pool_row] = row.scale;
   }
-  uint8_t* dst = a.codes + pool_row * HD;
-  *reinterpret_cast<uint2*>(dst + at_a) = make_uint2(words[0], words[1]);
-  *reinterpret_cast<uint2*>(dst + at_b) = make_uint2(words[2], words[3]);
-  if (sub == 0) a.scales[pool_row] = row.scale;
 }
 
-// Sixteen codes as values of T.
+// Sixteen codes as values of T: exact as halves, times the scale in float32.
+__device__ __forceinline__ void store_pair(float* out, float2 v) { *reinterpret_cast<float2*>(out) = v; }
+__device__ __forceinline__ void store_pair(__nv_bfloat16* out, float2 v) {
+  *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(v.x, v.y);
+}
 template <typename T, int KIND> __device__ __forceinline__ void code_values(const uint4& word, float scale, T* out) {
-  const uint32_t w[4] = {word.x, word.y, word.z, word.w};
+  const uint32_t words[4] = {word.x, word.y, word.z, word.w};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) out[i] = from_float<T>(code_value<KIND>((w[i >> 2] >> (8 * (i & 3))) & 0xffu) * scale);
+  for (int w = 0; w < 4; ++w) {
+    uint32_t halves[2];
+    code_halves<KIND>(words[w], halves[0], halves[1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&halves[h]));
+      store_pair(out + 4 * w + 2 * h, make_float2(v.x * scale, v.y * scale));
+    }
+  }
 }
 
 // Pages back into the compute type, for rows of whole 16-byte pieces: a page's
@@ -307,7 +316,7 @@ template <typename T, int KIND> __device__ __forceinline__ void code_values(cons
 // kReadPieces pieces of one page at a time, each thread all its loads in flight
 // before the first store. Block (x, request) takes the items x, x + gridDim.x, ...
 // of the request's walk over the pages that are seen.
-constexpr int kReadThreads = 256, kReadDepth = 4, kReadPieces = kReadThreads * kReadDepth;
+constexpr int kReadThreads = 256, kReadDepth = 2, kReadPieces = kReadThreads * kReadDepth;
 constexpr int kReadBlocks = 8 * 148 * 8;   // of a launch, at most (or one a request): eight rounds of what is resident
 
 template <typename T, int KIND>
