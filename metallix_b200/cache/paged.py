@@ -14,7 +14,10 @@ reference keeps K and V per layer as ``[slots, kv_heads, head_dim]``
 (crates/models/qwen/src/forward/paged.rs:135-146); here a head's rows of one
 page are contiguous so that a kernel reads a page of one head as one block.
 State entries are ``[request_slots, *state_shape]``, zeroed when a request is
-admitted. A mixer made of mixers has one need per member; each gets memory of
+admitted. Groups whose need says ``codes`` hold 8-bit codes in that layout and a
+float32 scale per row beside them; pages are read back, for the attention of
+prompts, into one buffer in the compute type per shape, ``[pages, planes,
+kv_heads, page_tokens, head_dim]``, that all entries share. A mixer made of mixers has one need per member; each gets memory of
 its own under the key ``(entry, member index)``.
 """
 from __future__ import annotations
@@ -37,11 +40,14 @@ class Group:
     page_tokens: int
     num_pages: int
     pool: Optional[torch.Tensor]  # [entries, pages, 2, kv_heads, page_tokens, head_dim]
+    scales: Optional[torch.Tensor] = None   # with codes: [entries, pages, 2, kv_heads, page_tokens]
+    values: Optional[torch.Tensor] = None   # with codes: where an entry's pages are read back
 
     def bytes_per_page(self) -> int:
         if self.pool is None:
             return 0
-        return self.pool[0, 0].numel() * self.pool.element_size() * len(self.entries)
+        scales = 0 if self.scales is None else self.scales[0, 0].numel() * self.scales.element_size()
+        return (self.pool[0, 0].numel() * self.pool.element_size() + scales) * len(self.entries)
 
 
 class PagedCache:
@@ -53,9 +59,16 @@ class PagedCache:
         entries: what a pool of n pages per group costs is n times this. The
         reference sizes its pool from a byte budget the same way
         (crates/core/engine/src/blocks.rs:162-180)."""
+        pages = [need for whole in needs if whole is not None for need in whole.flat() if need.kind == "kv_pages"]
         size = torch.empty((), dtype=dtype).element_size()
-        return sum(need.planes * need.kv_heads * need.head_dim * page_tokens * size
-                   for whole in needs if whole is not None for need in whole.flat() if need.kind == "kv_pages")
+        read_back = {(need.planes, need.kv_heads, need.head_dim) for need in pages if need.codes}   # one buffer per shape
+        return page_tokens * (sum(need.planes * need.kv_heads * PagedCache._row_bytes(need, size) for need in pages)
+                              + sum(planes * heads * dim * size for planes, heads, dim in read_back))
+
+    @staticmethod
+    def _row_bytes(need: CacheNeed, size: int) -> int:
+        """Bytes of one row of a page: its values of ``size`` bytes, or its codes and their scale."""
+        return need.head_dim + 4 if need.codes else need.head_dim * size
 
     def __init__(self, needs: Sequence[Optional[CacheNeed]], page_tokens: int, num_pages: int,
                  max_requests: int, dtype: torch.dtype, device, allocate: bool = True):
@@ -104,10 +117,18 @@ class PagedCache:
             [host.GroupConfig(page_tokens, g.need.window or 0, g.num_pages, g.need.chunk or 0, g.need.keep) for g in self.groups],
             max_requests)
         if allocate:
+            from ..ops import CODE_DTYPES
+            read_back: Dict[tuple, torch.Tensor] = {}
             for group in self.groups:
-                group.pool = torch.zeros(
-                    (len(group.entries), group.num_pages, group.need.planes, group.need.kv_heads, page_tokens,
-                     group.need.head_dim), dtype=dtype, device=self.device)
+                shape = (group.num_pages, group.need.planes, group.need.kv_heads, page_tokens, group.need.head_dim)
+                codes = group.need.codes
+                group.pool = torch.zeros((len(group.entries),) + shape, dtype=CODE_DTYPES[codes] if codes else dtype,
+                                         device=self.device)
+                if codes:
+                    group.scales = torch.zeros((len(group.entries),) + shape[:-1], dtype=torch.float32, device=self.device)
+                    if shape not in read_back:
+                        read_back[shape] = torch.zeros(shape, dtype=dtype, device=self.device)
+                    group.values = read_back[shape]
 
     @staticmethod
     def _members(need: CacheNeed, path: tuple = ()):
@@ -122,10 +143,11 @@ class PagedCache:
     def bytes_per_token(self) -> int:
         """Bytes of keys and values one position takes over all groups."""
         size = torch.empty((), dtype=self.dtype).element_size()
-        return sum(g.need.planes * g.need.kv_heads * g.need.head_dim * size * len(g.entries) for g in self.groups)
+        return sum(g.need.planes * g.need.kv_heads * self._row_bytes(g.need, size) * len(g.entries) for g in self.groups)
 
     def pool_bytes(self) -> int:
-        return sum(g.pool.numel() * g.pool.element_size() for g in self.groups if g.pool is not None)
+        held = {t.data_ptr(): t for g in self.groups for t in (g.pool, g.scales, g.values) if t is not None}
+        return sum(t.numel() * t.element_size() for t in held.values())
 
     # ------------------------------------------------------------------- fork
     def fork(self, parent: int, child: int) -> None:
@@ -138,8 +160,8 @@ class PagedCache:
         source_slot, target_slot, copies = self.manager.fork(parent, child)
         if self.device.type != "cuda":
             return
-        ops.copy_units_by_host([(self.groups[g].pool, source, target) for g, source, target in copies
-                                if self.groups[g].pool is not None]
+        ops.copy_units_by_host([(held, source, target) for g, source, target in copies
+                                for held in (self.groups[g].pool, self.groups[g].scales) if held is not None]
                                + [(state, source_slot, target_slot) for state in self._state_units])
 
     # ------------------------------------------------------------- step views
@@ -166,6 +188,10 @@ class PagedCache:
         if need.kind == "state":
             return CacheView(need=need, state=self.states[entry], write=write)
         group = self.groups[self.entry_group[entry]]
-        return CacheView(need=need, pool=group.pool[self.entry_index[entry]],
-                         block_tables=tables[group.index],
-                         slots=slots[group.index] if write else None, write=write)
+        index = self.entry_index[entry]
+        pool = group.pool[index]
+        if group.scales is not None:
+            from ..ops import QuantizedPool
+            pool = QuantizedPool(pool, group.scales[index])
+        return CacheView(need=need, pool=pool, block_tables=tables[group.index],
+                         slots=slots[group.index] if write else None, write=write, values=group.values)

@@ -85,6 +85,8 @@ class CacheNeed:
     ever read again; the first ``keep`` positions of a sequence are kept beside
     either. ``planes`` is 2 for keys and values, 1 for a pool with
     one row per position that serves as both (a latent that all heads share).
+    ``codes`` ("fp8", "int8") says that the rows are held as 8-bit codes with a
+    scale each, because the engine was asked for it and the mixer can read them.
     ``kind == "state"``: ``state_shape`` values of fixed
     size per request, zeroed when the request is admitted. ``kind == "none"``:
     the mixer keeps nothing between steps. ``kind == "several"``: a mixer made
@@ -101,10 +103,11 @@ class CacheNeed:
     planes: int = 2
     members: Tuple["CacheNeed", ...] = ()
     keep: int = 0
+    codes: Optional[str] = None
 
     def group_key(self) -> tuple:
         return (self.kind, self.kv_heads, self.head_dim, self.window, self.chunk, self.keep,
-                tuple(self.state_shape), self.state_dtype, self.planes,
+                tuple(self.state_shape), self.state_dtype, self.planes, self.codes,
                 tuple(member.group_key() for member in self.members))
 
     def flat(self) -> Tuple["CacheNeed", ...]:

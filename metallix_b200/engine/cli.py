@@ -61,6 +61,8 @@ def build_parser() -> argparse.ArgumentParser:
     gen.add_argument("--top-k", type=int, default=0)
     gen.add_argument("--sampler", choices=("icdf", "race"), default="icdf")
     gen.add_argument("--dtype", choices=("bfloat16", "float32"), default="bfloat16")
+    gen.add_argument("--cache-dtype", choices=("auto", "fp8", "int8"), default="auto",
+                     help="how keys and values are cached: as computed, or as 8-bit codes with a scale per position and head")
     gen.add_argument("--block-size", type=int, default=16, help="positions per cache page")
     gen.add_argument("--num-pages", type=int, help="pages of the cache pool")
     gen.add_argument("--kv-pool-mib", type=int, help="size the cache pool by bytes instead")
@@ -144,7 +146,7 @@ def run_gen(args) -> int:
     from .generate import generate
 
     started = time.perf_counter()
-    options = dict(dtype=args.dtype, page_tokens=args.block_size, gemm_backend=args.gemm,
+    options = dict(dtype=args.dtype, page_tokens=args.block_size, gemm_backend=args.gemm, cache_dtype=args.cache_dtype,
                    max_requests=max(args.max_num_seqs, 1) + 1)
     if args.model:
         from ..config import read_config

@@ -74,12 +74,18 @@ class Engine:
                  max_context: Optional[int] = None, device="cuda:0", gemm_backend: str = "auto",
                  spec=None, cuda_graphs: bool = True, chained_launches: bool = True,
                  pool_bytes: Optional[int] = None, pool_fraction: Optional[float] = None,
-                 consume_tensors: bool = False):
+                 consume_tensors: bool = False, cache_dtype: Optional[str] = None):
         """The cache pool is sized by the first of these that is given:
         ``num_pages``; ``max_tokens`` (positions all live requests may hold);
         ``pool_bytes``; ``pool_fraction`` of the device memory that is free
         once the weights are resident (what a large model on one GPU wants);
-        else four contexts of up to 4,096 positions."""
+        else four contexts of up to 4,096 positions.
+
+        ``cache_dtype``: None (or "auto") keeps keys and values in the compute
+        type; "fp8" (e4m3) and "int8" keep them as 8-bit codes with a float32
+        scale per position and head, half the bytes that a bfloat16 decode step
+        reads. Only grouped-query attention reads codes: a model with another
+        mixer that caches rows per position is refused."""
         ops.require_cuda()
         self.chained_launches = bool(chained_launches)
         ops.set_chained_launches(self.chained_launches)
@@ -93,9 +99,15 @@ class Engine:
             # anything torch may run on this path.
             torch.backends.cuda.matmul.allow_tf32 = False
             torch.backends.cudnn.allow_tf32 = False
+        if cache_dtype not in (None, "auto", *ops.CODE_DTYPES):
+            raise ValueError(f"cache_dtype must be auto, fp8 or int8, got {cache_dtype!r}")
+        self.cache_dtype = None if cache_dtype == "auto" else cache_dtype
         self.runtime = Runtime(device=self.device, dtype=self.dtype, max_positions=self.max_context,
-                               gemm_backend=gemm_backend)
+                               gemm_backend=gemm_backend, cache_codes=self.cache_dtype)
         self.model = DecoderModel(self.spec, tensors, self.runtime, consume=consume_tensors)
+        if self.cache_dtype and not all(need.codes for whole in self.model.cache_needs() if whole is not None
+                                        for need in whole.flat() if need.kind == "kv_pages"):
+            raise ValueError(f"cache_dtype {cache_dtype!r}: the model has a mixer whose rows are cached in the compute type only")
         if num_pages is None and max_tokens is None and (pool_bytes is not None or pool_fraction is not None):
             if pool_bytes is None:
                 if not 0.0 < pool_fraction <= 1.0:

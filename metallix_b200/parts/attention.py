@@ -103,6 +103,8 @@ def attention_tiles(plan: StepPlan) -> Prepared:
     token, for the split-key kernel (a negative token is a padding row).
     ``wide_*``: tiles of up to 128 tokens over the requests that bring
     several, those with most keys first, for the tensor-core prompt kernels.
+    ``read_*``: the requests that bring several tokens, their first and last
+    positions, for caches whose pages are read back first.
     Facts: ``longest_context`` bounds position + 1 of the single tokens,
     ``longest_keys`` the keys a wide tile sees. A portion of a prompt behind
     ``LONG_CONTEXT`` keys or more runs other launches (its keys are shared out
@@ -116,13 +118,14 @@ def attention_tiles(plan: StepPlan) -> Prepared:
         arrays = {"tile_request": index, "tile_start": index, "tile_length": alive.astype(np.int32),
                   "decode_token": np.where(alive, index, -1).astype(np.int32), "decode_request": index}
         empty = np.empty(0, dtype=np.int32)
-        arrays.update(wide_request=empty, wide_start=empty, wide_length=empty)
+        arrays.update(wide_request=empty, wide_start=empty, wide_length=empty, read_request=empty, read_first=empty,
+                      read_last=empty)
         longest = plan.context_bound if plan.replayable else max(
             [starts[row] + 1 for row in range(min(live, rows))], default=1)
         return Prepared(arrays, {"multi_tiles": 0, "decode_rows": rows, "longest_context": longest,
                                  "longest_keys": 0}, graph_key=False)
     tile_request, tile_start, tile_length = [], [], []
-    singles, wide = [], []
+    singles, wide, read = [], [], []
     longest, longest_keys, begin = 0, 0, 0
     for row, (count, start) in enumerate(zip(counts, starts)):
         if count == 1:
@@ -134,6 +137,7 @@ def attention_tiles(plan: StepPlan) -> Prepared:
                 tile_start.append(begin + first)
                 tile_length.append(min(TILE_TOKENS, count - first))
             longest_keys = max(longest_keys, start + count)
+            read.append((row, start, start + count - 1))
             for first in range(0, count, WIDE_TOKENS):
                 size = min(WIDE_TOKENS, count - first)
                 wide.append((start + first + size, row, begin + first, size))
@@ -154,7 +158,8 @@ def attention_tiles(plan: StepPlan) -> Prepared:
               "decode_token": as_array([token if length else -1 for _, token, length in singles]),
               "decode_request": as_array([row for row, _, _ in singles]),
               "wide_request": as_array([w[1] for w in wide]), "wide_start": as_array([w[2] for w in wide]),
-              "wide_length": as_array([w[3] for w in wide])}
+              "wide_length": as_array([w[3] for w in wide]), "read_request": as_array([r[0] for r in read]),
+              "read_first": as_array([r[1] for r in read]), "read_last": as_array([r[2] for r in read])}
     return Prepared(arrays, {"multi_tiles": multi_tiles, "decode_rows": len(singles), "longest_context": longest,
                              "longest_keys": longest_keys}, graph_key=many_keys)
 
@@ -190,8 +195,12 @@ def attend_cached(q_heads: torch.Tensor, cache: CacheView, ctx: StepContext, *, 
     as (float32 ``[heads, tokens, hidden]`` summands, True), merged and
     projected by one kernel. ``split_decode`` and ``flash`` say which of the first
     two the caller lets its requests take. ``key_width`` / ``value_width``: how many
-    values of a head's keys and values are in use (0: all), the others being zeros."""
+    values of a head's keys and values are in use (0: all), the others being zeros.
+    Of a cache held as codes, single tokens read the codes, which takes
+    ``split_decode``; for portions of prompts the pages that they see are read back
+    into the compute type first."""
     tokens, heads, head_dim = q_heads.shape
+    coded = isinstance(cache.pool, ops.QuantizedPool)
     if flash and head_dim == 256:
         # Such heads have a prompt kernel for some page sizes only; it reads a gate 16 bytes at a time and takes a row's
         # maximum ahead of the scaling.
@@ -209,17 +218,24 @@ def attend_cached(q_heads: torch.Tensor, cache: CacheView, ctx: StepContext, *, 
         return ops.paged_attention_decode_project(
             q_heads, cache.pool, cache.block_tables, tiles["decode_token"], tiles["decode_request"],
             ctx.positions, scale, tiles["longest_context"], project.weight, window, chunk, gate=gate,
-            softcap=softcap, sink=sink, bias=bias, keep=keep), True
+            softcap=softcap, sink=sink, bias=bias, keep=keep, settled=True), True
     out = torch.empty_like(q_heads)
     if split:
         # Requests that bring one token: split along the keys.
         ops.paged_attention_decode(q_heads, cache.pool, out, cache.block_tables, tiles["decode_token"],
                                    tiles["decode_request"], ctx.positions, scale, tiles["longest_context"], window,
-                                   chunk=chunk, gate=gate, softcap=softcap, sink=sink, bias=bias, keep=keep)
+                                   chunk=chunk, gate=gate, softcap=softcap, sink=sink, bias=bias, keep=keep, settled=True)
+    pool = cache.pool
+    if coded:
+        if tiles["decode_rows"] and not split:
+            raise ValueError("single tokens over a cache held as codes need the split-key decode kernel")
+        if tiles["read_request"].numel():
+            pool = ops.read_cache(cache.pool, cache.values, cache.block_tables, tiles["read_request"], tiles["read_first"],
+                                  tiles["read_last"], window=window, chunk=chunk, keep=keep)
     if flash:
         # Requests that bring several tokens: tensor cores, tiles of 128.
         if tiles["wide_request"].numel():
-            ops.flash_prefill(q_heads, cache.pool, out, cache.block_tables, tiles["wide_request"],
+            ops.flash_prefill(q_heads, pool, out, cache.block_tables, tiles["wide_request"],
                               tiles["wide_start"], tiles["wide_length"], ctx.positions, scale, window,
                               longest_context=tiles["longest_keys"], chunk=chunk, gate=gate, softcap=softcap,
                               sink=sink, bias=bias, keep=keep, key_width=key_width, value_width=value_width)
@@ -227,7 +243,7 @@ def attend_cached(q_heads: torch.Tensor, cache: CacheView, ctx: StepContext, *, 
     else:
         rest = slice(0, multi_tiles) if split else slice(0, None)
     if rest is not None and tiles["tile_request"][rest].numel():
-        ops.paged_attention_tile(q_heads, cache.pool, out, cache.block_tables, tiles["tile_request"][rest],
+        ops.paged_attention_tile(q_heads, pool, out, cache.block_tables, tiles["tile_request"][rest],
                                  tiles["tile_start"][rest], tiles["tile_length"][rest], ctx.positions,
                                  scale, window, chunk, gate=gate, softcap=softcap, gate_per_head=gate_per_head,
                                  sink=sink, bias=bias, keep=keep)
@@ -410,17 +426,21 @@ class GQAttention:
         # What only the general kernel does: values of another width than the keys.
         self.general_only = self.value_dim != self.head_dim
         self.fused = norms_fuse and eps_agree and position_fuses and self.value_dim == self.head_dim
-        self.split_decode = not self.general_only and ops.decode_attention_supported(
+        self.codes = runtime.cache_codes
+        if self.codes and self.general_only:
+            raise ValueError("values of another width than the keys are cached in the compute type only")
+        self.split_decode = not self.general_only and (ops.quantized_decode_supported if self.codes else ops.decode_attention_supported)(
             self.head_dim, self.num_heads, self.num_kv_heads, self.dtype)
         if self.split_decode and self.dtype == torch.float32:
             runtime.ordered_sums = False
         # heads of 256 values: attend_cached asks whether the kernel takes the cache's pages
         self.flash = not self.general_only and (ops.flash_prefill_supported(
-            self.head_dim, self.num_heads, self.num_kv_heads, self.dtype) or (self.split_decode and self.head_dim == 256))
+            self.head_dim, self.num_heads, self.num_kv_heads, self.dtype) or (
+                self.head_dim == 256 and ops.decode_attention_supported(256, self.num_heads, self.num_kv_heads, self.dtype)))
 
     def cache_need(self) -> CacheNeed:
         return CacheNeed(kind="kv_pages", kv_heads=self.num_kv_heads, head_dim=self.row_dim,
-                         window=self.window or None, chunk=self.chunk or None, keep=self.keep)
+                         window=self.window or None, chunk=self.chunk or None, keep=self.keep, codes=self.codes)
 
     def parts(self):
         return [self.q_norm, self.k_norm, self.position, self.value_position]

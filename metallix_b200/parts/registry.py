@@ -56,6 +56,8 @@ class Runtime:
     # How bfloat16 matrix products run: auto | tcgen05 | cublas | simple. In float32 anything but auto means the general
     # product in ascending order throughout.
     gemm_backend: str = "auto"
+    # How mixers that can are to hold their keys and values: None (the compute type), "fp8" or "int8" (8-bit codes).
+    cache_codes: Optional[str] = None
     # Read-only tensors that parts built from equal parameters may share
     # (tables of a position encoding, say), by a key of those parameters.
     shared: Dict[tuple, object] = field(default_factory=dict)
@@ -108,18 +110,22 @@ class CacheView:
     For ``kv_pages`` entries: ``pool`` is this entry's
     ``[pages, 2, kv_heads, page_tokens, head_dim]`` tensor, ``block_tables``
     ``[requests, max_pages]`` and ``slots`` ``[tokens]`` belong to the entry's
-    group (``slots`` is None when the run may not write). For ``state``
+    group (``slots`` is None when the run may not write); where the need says
+    ``codes``, ``pool`` is a ``QuantizedPool`` and ``values`` a tensor of its shape
+    in the compute type, which every entry of that shape shares, for pages read
+    back. For ``state``
     entries: ``state`` is ``[request_slots, *state_shape]``, indexed by
     ``StepContext.request_slots``.
     """
 
     need: CacheNeed
-    pool: Optional[torch.Tensor] = None
+    pool: Optional[torch.Tensor] = None      # or an ops.QuantizedPool
     block_tables: Optional[torch.Tensor] = None
     slots: Optional[torch.Tensor] = None
     state: Optional[torch.Tensor] = None
     write: bool = True
     members: Sequence["CacheView"] = ()
+    values: Optional[torch.Tensor] = None
 
 
 @dataclass
