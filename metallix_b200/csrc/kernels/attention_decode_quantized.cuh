@@ -269,8 +269,20 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
   if (!release_late) chain_release();
   const int rank = blockIdx.x, slots = gridDim.x, kv = blockIdx.y % a.kv_heads, part = blockIdx.y / a.kv_heads, row = blockIdx.z;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  // Pages are a power of two of 8 positions or more: a box is a page's rows of one plane, or of a stage where a page has more.
+  // Lane n has box n fetched (keys' boxes, then values'; for heads of 256 each as two halves) and looks after key n's scales.
+  // Pages are asked for one stage ahead of the copies, and looked at only then; those of the first stage together with the
+  // position, on the guess that neither a window nor a chunk has moved the first tile.
+  constexpr int WIDE = HD / Tile::kBoxBytes;   // boxes a row is cut into
+  const int shift = a.page_shift, in_page = a.page_tokens - 1, box_keys = min(a.page_tokens, KEYS);
+  const int per_plane = KEYS / box_keys, boxes = 2 * per_plane * WIDE;
+  const int plane = lane / (per_plane * WIDE), box = lane % (per_plane * WIDE) / WIDE, wide = lane % WIDE;
+  const int box_key = box * box_keys, scale_key = lane % KEYS;
   if (!a.settled) chain_wait();
   const int token = a.row_token[row];
+  const int* table = a.block_tables + static_cast<size_t>(a.row_request[row]) * a.max_pages;
+  auto page_at = [&](int key) { return (key >> shift) < a.max_pages ? table[key >> shift] : -1; };
+  int box_page = page_at(rank * kSplitKeys + warp * 32 + box_key), scale_page = page_at(rank * kSplitKeys + warp * 32 + scale_key);
   if (token < 0) return;   // a padding row
   const int pos = a.positions[token], group = a.heads / a.kv_heads;
   const int live = min(group - part * 8, 8), head0 = kv * group + part * 8;   // this block's query heads
@@ -313,7 +325,6 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
     }
     return;
   }
-  const int* table = a.block_tables + static_cast<size_t>(a.row_request[row]) * a.max_pages;
   unsigned char* ring = quant_shared + warp * Tile::kWarpBytes;
   float* ring_scales = reinterpret_cast<float*>(quant_shared + WARPS * Tile::kWarpBytes) + warp * (STAGES * Tile::kScales);
   uint64_t* landed = barriers + warp * STAGES;
@@ -329,17 +340,7 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
   auto first_of = [&](int i) { return walk.tile(rank + i / HALVES * slots) * kSplitKeys + warp * 32 + i % HALVES * KEYS; };
   auto holds = [&](int key0) { return key0 <= pos && (key0 + KEYS > first_key || key0 < a.keep); };
   auto wanted = [&](int key, int keys) { return key <= pos && (key + keys > first_key || key < a.keep); };
-  // Pages are a power of two of 8 positions or more: a box is a page's rows of one plane, or of a stage where a page has more.
-  // Lane n has box n fetched (keys' boxes, then values'; for heads of 256 each as two halves) and looks after key n's scales.
-  // Pages are asked for one stage ahead of the copies, and looked at only then.
-  const int shift = a.page_shift, in_page = a.page_tokens - 1, box_keys = min(a.page_tokens, KEYS);
-  constexpr int WIDE = HD / Tile::kBoxBytes;   // boxes a row is cut into
-  const int per_plane = KEYS / box_keys, boxes = 2 * per_plane * WIDE;
-  const int plane = lane / (per_plane * WIDE), box = lane % (per_plane * WIDE) / WIDE, wide = lane % WIDE;
-  auto page_of = [&](int i, int key) {   // the page of key `key` of stage i, as the table has it
-    const int slot = (first_of(i) + key) >> shift;
-    return i < stages && slot < a.max_pages ? table[slot] : -1;
-  };
+  auto page_of = [&](int i, int key) { return i < stages ? page_at(first_of(i) + key) : -1; };   // of key `key` of stage i
   const int value_rows = a.kv_heads * a.page_tokens;   // from a key's row to its value's
   auto row_in = [&](int page, int key) { return (page * 2 * a.kv_heads + kv) * a.page_tokens + (key & in_page); };
   // Every box of a stage is fetched: one that holds nothing the token sees starts behind the pool's last row, where the
@@ -376,8 +377,10 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
   // The token's own row, of the walk's last tile, is written by the kernel ahead of this one; with `settled` all others
   // are older, and their copies start ahead of the wait.
   bool waited = !a.settled;
-  const int box_key = box * box_keys, scale_key = lane % KEYS;
-  int box_page = page_of(0, box_key), scale_page = page_of(0, scale_key);
+  if (walk.tile(rank) != rank) {
+    box_page = page_of(0, box_key);
+    scale_page = page_of(0, scale_key);
+  }
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) {
     if (!waited && i < stages && first_of(i) + KEYS > pos) {
