@@ -296,7 +296,8 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
   // [8 heads][HD + 2] with maxima in powers of two, and a block writes every slots-th part of the output.
   float* results = reinterpret_cast<float*>(quant_shared) + WARPS * 8 * (HD + 2);
   auto finish = [&]() {
-    quant_cluster_sync();
+    if (slots > 1) quant_cluster_sync();
+    else __syncthreads();
     const int parts_in = min(slots, walk.count);   // the others have nothing
     for (int i = rank * kDecodeThreads + threadIdx.x; i < live * HD; i += slots * kDecodeThreads) {
       const int h = i / HD, d = i - h * HD;
@@ -316,7 +317,7 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
       }
       static_cast<T*>(a.out)[(static_cast<size_t>(token) * a.heads + head) * HD + d] = from_float<T>(value);
     }
-    quant_cluster_sync();   // nobody leaves while its results are being read
+    if (slots > 1) quant_cluster_sync();   // nobody leaves while its results are being read
   };
   if (rank >= walk.count) {   // more slots than tiles
     if (a.fused) {
@@ -675,7 +676,7 @@ static cudaError_t launch_quantized_mma(const QuantizedDecode& args, dim3 grid, 
   if (!encode_codes_map(&map, args.codes, static_cast<long long>(args.num_pages) * 2 * args.kv_heads * args.page_tokens, HD,
                         args.page_tokens < keys ? args.page_tokens : keys))
     return cudaErrorInvalidValue;
-  if (args.fused) return launch_chained_clusters(kernel, grid, dim3(kDecodeThreads), QuantTile<HD>::kShared, grid.x, stream, map, args);
+  if (args.fused && grid.x > 1) return launch_chained_clusters(kernel, grid, dim3(kDecodeThreads), QuantTile<HD>::kShared, grid.x, stream, map, args);
   return launch_chained(kernel, grid, dim3(kDecodeThreads), QuantTile<HD>::kShared, stream, map, args);
 }
 
@@ -697,7 +698,7 @@ static cudaError_t launch_quantized_decode(QuantizedDecode args, int kind, int r
     if (fusable && count > kQuantCluster && tiles <= 6 * kQuantCluster && kQuantCluster * pairs <= resident) count = kQuantCluster;
     // Clusters only where all blocks are resident at once: in further rounds a cluster waits for as many places side by side
     // (37 requests of 7,000 positions in three blocks a pair: 115 us as clusters, 92 without).
-    args.fused = fusable && count <= kQuantCluster && static_cast<long long>(count) * pairs <= resident;
+    args.fused = fusable && (count == 1 || (count <= kQuantCluster && static_cast<long long>(count) * pairs <= resident));
     if (!args.fused && args.partial == nullptr) return cudaErrorNotReady;   // the caller is to bring room for the partial results
     *slots = args.fused ? 0 : count;
     const dim3 grid(count, args.kv_heads * parts, rows);

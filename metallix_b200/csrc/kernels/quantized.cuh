@@ -88,26 +88,42 @@ __device__ __forceinline__ float odd_quotient(float x, const RowScale& r) {
   return y;
 }
 
-// Four values' codes as the bytes of a word.
-template <int KIND> __device__ __forceinline__ uint32_t four_codes(const float* x, const RowScale& r) {
-  if (r.inverse == 0.0f) return 0u;   // a row of zeros, or one that is not finite
-  float y[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) y[j] = odd_quotient(x[j], r);
+// Four quotients' codes as the bytes of a word.
+template <int KIND> __device__ __forceinline__ uint32_t round_to_codes(const float* y) {
   if (KIND == kCodesE4M3) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
   }
-  if (r.shift != 1.0f) {   // scales among the smallest numbers are coarse: their quotients may lie beyond 127.5
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = fminf(fmaxf(y[j], -127.0f), 127.0f);
-  }
-  // to the nearest even by the sum's own rounding: |y| is at most 127 and an ulp, and the low byte is the code's
+  // to the nearest even by the sum's own rounding: |y| is below 127.5, and the low byte is the code's
   uint32_t c[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) c[j] = __float_as_uint(__fadd_rn(y[j], 12582912.0f));   // 1.5 x 2^23
   return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+
+// Four values' codes as the bytes of a word. The product by the reciprocal is within 2^-23 of the quotient, so if both ends
+// of the numbers within 2^-21 of it have one code that is the quotient's; else (one value in 10^5, and rows whose scale is a
+// power of two) the quotient is rounded to odd first. Five instructions a value instead of fourteen.
+template <int KIND> __device__ __forceinline__ uint32_t four_codes(const float* x, const RowScale& r) {
+  if (r.inverse == 0.0f) return 0u;   // a row of zeros, or one that is not finite
+  float below[4], beyond[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float y = x[j] * r.inverse;
+    below[j] = y * (1.0f - 0x1p-21f);
+    beyond[j] = y * (1.0f + 0x1p-21f);
+  }
+  const uint32_t codes = round_to_codes<KIND>(below);
+  if (codes == round_to_codes<KIND>(beyond) && r.shift == 1.0f) return codes;
+  float y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    y[j] = odd_quotient(x[j], r);
+    // scales among the smallest numbers are coarse: their quotients may lie beyond 127.5
+    if (KIND == kCodesInt8) y[j] = fminf(fmaxf(y[j], -127.0f), 127.0f);
+  }
+  return round_to_codes<KIND>(y);
 }
 
 template <int KIND> __device__ __forceinline__ uint32_t code_of(float x, const RowScale& r) {
@@ -118,6 +134,12 @@ template <int KIND> __device__ __forceinline__ uint32_t code_of(float x, const R
 }
 
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// The larger magnitude, or NaN where either is one.
+__device__ __forceinline__ float larger_magnitude(float x, float y) {
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(z) : "f"(fabsf(x)), "f"(fabsf(y)));
+  return z;
+}
 
 // Which row of the pool position `key` of a request lies in, counted over
 // [pages, page_tokens] of one plane and head: (page * 2 * kv_heads + kv) *

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(256) store_quantized_kernel(const StoreArgs a)
 // the values behind the rotated ones); either way the lane needs the cosines
 // 8 s ... 8 s + 7. Issue slots and the wait for positions, cosines and rows bind
 // it, so warps of queries end at their rotation (2,048 tokens of 32 / 8 heads of
-// 128: 20.6 us when they took the codes' part too, 18.0; the write of the same
+// 128: 20.6 us when they took the codes' part too, 17.6; the write of the same
 // rows in bfloat16 takes 14.5). Two or four heads a lane with one set of weights
 // and cosines, as that write does it, lose more warps than they save loads
 // (20.5 and 22.4 us).
@@ -278,13 +278,14 @@ __global__ void __launch_bounds__(256) store_quantized_lanes_kernel(const __grid
     }
   }
   if (!__any_sync(0xffffffffu, active && !is_q)) return;   // a warp of queries
-  uint32_t largest = 0;
+  float largest = x[0];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) largest = max(largest, magnitude_bits(x[j]));
+  for (int j = 1; j < 16; ++j) largest = larger_magnitude(largest, x[j]);
 #pragma unroll
-  for (int offset = LANES / 2; offset > 0; offset >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
+  for (int offset = LANES / 2; offset > 0; offset >>= 1)
+    largest = larger_magnitude(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
   if (active && !is_q) {
-    const RowScale row = row_scale<KIND>(largest);
+    const RowScale row = row_scale<KIND>(__float_as_uint(largest));
     uint8_t* dst = a.codes + pool_row * HD;
     *reinterpret_cast<uint2*>(dst + at_a) = make_uint2(four_codes<KIND>(x, row), four_codes<KIND>(x + 4, row));
     *reinterpret_cast<uint2*>(dst + at_b) = make_uint2(four_codes<KIND>(x + 8, row), four_codes<KIND>(x + 12, row));
