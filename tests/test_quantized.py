@@ -431,6 +431,50 @@ def test_decode_options(ops, dtype, head_dim, heads, kv_heads, page, options):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim,heads,kv_heads,page,rows,longest", [
+    (128, 8, 4, 16, 45, 2500), (64, 12, 4, 32, 120, 1100), (256, 4, 4, 16, 30, 3000), (128, 24, 2, 8, 70, 1500), (64, 8, 8, 64, 200, 1025),
+    (128, 4, 4, 16, 520, 1100), (128, 8, 8, 16, 9, 40000)])
+@pytest.mark.parametrize("options", [dict(), dict(window=900, softcap=4.0, sink="heads", keep=130, gate=True)],
+                         ids=["bare", "options"])
+def test_decode_of_many_rows(ops, dtype, head_dim, heads, kv_heads, page, rows, longest, options):
+    """Batches of many pairs, in one round of blocks and in several: contexts from one position to the longest in any order, padding rows
+    between, one row beyond the bound on the contexts."""
+    rng = torch.Generator().manual_seed(rows)
+    lengths = torch.randint(1, longest + 1, (rows,), generator=rng).tolist()
+    lengths[rows // 2], lengths[1], lengths[2] = longest, 1, 128
+    pages, table = spread_tables(lengths, page, 5)
+    pool = random_pool(ops, "int8" if head_dim == 64 else "fp8", pages, kv_heads, page, head_dim, 6)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn((rows + 1, heads, head_dim), generator=gen, device="cuda").to(dtype)
+    positions = ints([n - 1 for n in lengths] + [longest + 300])
+    options = dict(options)
+    if options.get("sink") == "heads":
+        options["sink"] = torch.randn(heads, generator=gen, device="cuda")
+    if options.get("gate"):
+        options["gate"] = torch.randn((rows + 1, heads * head_dim), generator=gen, device="cuda").to(dtype)
+    order = torch.randperm(rows, generator=rng).tolist()
+    listed = [(t, t) for t in order]
+    for at in (0, rows // 3, len(listed)):
+        listed.insert(at, (-1, 0))
+    listed.insert(rows // 4, (rows, 0))       # beyond the bound: left as it is, and reported
+    out = torch.full(q.shape, 5.0, dtype=dtype, device="cuda")
+    scale = 1.0 / math.sqrt(head_dim)
+    for _ in range(2):
+        ops.paged_attention_decode(q, pool, out, table, ints([t for t, _ in listed]), ints([r for _, r in listed]), positions, scale,
+                                   longest, **options)
+    with pytest.raises(ops.KernelError, match="position"):
+        ops.check_status("cuda")
+    assert out[rows].eq(5.0).all()
+    some = list(range(rows)) if rows * longest < 200_000 else sorted({1, 2, rows // 2, 0, rows - 1, rows // 5, rows // 7})
+    exact, bound = exact_decode(q, pool, table, [(t, t) for t in some], positions, scale, **options)
+    if options.get("gate") is not None:
+        bound = bound * (1 + 1e-4)
+    close(out[some], exact[some], bound[some], dtype)
+    assert out[:rows].isfinite().all()
+
+
+@gpu
 @pytest.mark.parametrize("kind", ["fp8", "int8"])
 @pytest.mark.parametrize("head_dim,heads,kv_heads", [(128, 8, 2), (64, 7, 1)])
 def test_decode_with_the_output_projection(ops, kind, head_dim, heads, kv_heads):
@@ -497,3 +541,249 @@ def test_refusals_of_the_decode_attention(ops):
     for other in (ops.paged_attention_tile, ops.flash_prefill):      # the kernels that read a cache of the compute type say so
         with pytest.raises(ops.KernelError, match="cache must be a tensor"):
             other(q, pool, torch.zeros_like(q), ints([[0, 1]]), ints([0]), ints([0]), ints([1]), ints([3]), 0.1)
+
+
+# ----------------------------------------------------------------- numbers and calls at the edges
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("head_dim", [64, 128, 256, 40])
+def test_every_code_stands_for_its_number(ops, kind, head_dim):
+    """A context of one position gives its value back: every code, through the attention and through reading back."""
+    numbers = torch.arange(-127, 128).double() if kind == "int8" else \
+        torch.tensor([b for b in range(256) if b & 0x7f != 0x7f], dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    rows = -(-len(numbers) // head_dim)
+    values = torch.zeros(rows * head_dim, dtype=torch.float64)
+    values[:len(numbers)] = numbers
+    pool = ops.QuantizedPool.zeros(rows, 1, 8, head_dim, codes=kind)
+    pool.codes[:, 1, 0, 0] = values.view(rows, head_dim).to(pool.codes.dtype).cuda()
+    pool.scales[:, 1, 0, 0] = 2.0 ** -5
+    expect = (values.view(rows, 1, head_dim) * 2.0 ** -5).float().cuda()
+    for dtype in (F32, BF16):      # all of them have few enough bits for either type
+        q, out = (torch.ones(rows, 1, head_dim, device="cuda", dtype=dtype) for _ in range(2))
+        ops.paged_attention_decode(q, pool, out, ints([[r] for r in range(rows)]), ints(range(rows)), ints(range(rows)), ints([0] * rows),
+                                   0.1, 1)
+        assert torch.equal(out.float(), expect)
+        back = torch.zeros(pool.shape, dtype=dtype, device="cuda")
+        ops.read_cache(pool, back, ints([[r] for r in range(rows)]), ints(range(rows)), ints([0] * rows), ints([0] * rows))
+        assert torch.equal(back[:, 1, 0, 0].float(), expect[:, 0])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("q_size,k_size,v_size,spread", [(1e-30, 1.0, 1.0, 0), (1e30, 1e-25, 1.0, 0), (1.0, 40.0, 1e-30, 0), (1.0, 1.0, 1e30, 0),
+                                                         (1.0, 0.0, 1.0, 0), (30.0, 30.0, 1.0, 8), (1.0, 1.0, 1.0, 20)])
+def test_decode_of_far_sizes(ops, dtype, head_dim, q_size, k_size, v_size, spread):
+    """Queries, keys and values far from one; scores hundreds apart, in rising and falling order; values' scales that differ
+    from position to position by up to 2^spread. Weights below 2^-30 of the largest weight times scale are dropped."""
+    lengths, page = [777, 300], 16
+    pages, table = spread_tables(lengths, page, 8)
+    pool = random_pool(ops, "fp8", pages, 2, page, head_dim, 3)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    pool.scales[:, 0] *= k_size
+    pool.scales[:, 1] *= v_size
+    pool.scales[:, 1] *= torch.pow(2.0, (spread * torch.rand(pool.scales[:, 1].shape, generator=gen, device="cuda")).round())
+    for r, n in enumerate(lengths):       # keys that grow along the first context and shrink along the second
+        at = torch.arange(n)
+        grow = (at + 1.0) / n if r == 0 else 1.0 - at / n
+        pool.scales[table[r].cpu().long()[at // page].cuda(), 0, :, (at % page).cuda()] *= grow[:, None].cuda()
+    q = (q_size * torch.randn((2, 6, head_dim), generator=gen, device="cuda")).to(dtype)
+    out, positions = torch.zeros_like(q), ints([n - 1 for n in lengths])
+    ops.paged_attention_decode(q, pool, out, table, ints([0, 1]), ints([0, 1]), positions, 0.2, 777)
+    ops.check_status("cuda")
+    exact, bound = exact_decode(q, pool, table, [(0, 0), (1, 1)], positions, 0.2)
+    keys = pool.codes.float().abs().amax() * pool.scales[:, 0].nan_to_num().amax()
+    size = float(q.float().abs().amax() * keys * head_dim * 0.2)      # of a score, at most
+    largest = bound.amax(-1, keepdim=True)
+    per_weight = (HALF[BF16] if dtype == BF16 else 0.0) + max(size, 30) * 8 * 2.0 ** -24
+    limit = per_weight * bound + HALF[dtype] * exact.abs() * 1.01 + 2.0 ** -30 * 777 * largest
+    assert ((out.double() - exact).abs() <= limit).all()
+
+
+@gpu
+@pytest.mark.parametrize("offset", [1, 8])
+def test_operands_that_do_not_lie_on_16_bytes(ops, offset):
+    """Slices of larger tensors, which the vector forms do not take."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    aligned = random_pool(ops, "fp8", 9, 2, 16, 64, 1)
+    room = torch.zeros(aligned.codes.numel() + 16, dtype=torch.uint8, device="cuda")
+    codes = room[offset:offset + aligned.codes.numel()].view(torch.float8_e4m3fn).view(aligned.shape)
+    codes.view(torch.uint8).copy_(aligned.codes.view(torch.uint8))
+    pool = ops.QuantizedPool(codes, aligned.scales.clone())
+    table = ints([[3, 1, 7, 5, 0, 2, 8, 6, 4]])
+    k = torch.randn((3, 2 * 64 + 1), generator=gen, device="cuda").to(BF16)[:, 1:]
+    for p in (aligned, pool):
+        ops.write_cache(k, k, p, ints([3 * 16, 3 * 16 + 1, 7 * 16 + 4]), ints([0, 1, 36]))
+    assert torch.equal(pool.codes.view(torch.uint8), aligned.codes.view(torch.uint8)) and torch.equal(pool.scales, aligned.scales)
+    backs = [torch.zeros(pool.shape, dtype=BF16, device="cuda") for _ in range(2)]
+    for p, back in zip((aligned, pool), backs):
+        ops.read_cache(p, back, table, ints([0]), ints([100]), ints([100]))
+    assert torch.equal(*backs)
+    wide = torch.randn(1 * 4 * 64 + 8, generator=gen, device="cuda").to(BF16)
+    positions = ints([100])
+    for p, q in ((pool, wide[:256].view(1, 4, 64)), (aligned, wide[1:257].view(1, 4, 64))):
+        out = torch.zeros(1, 4, 64, dtype=BF16, device="cuda")
+        ops.paged_attention_decode(q, p, out, table, ints([0]), ints([0]), positions, 0.125, 101)
+        close(out, *exact_decode(q, p, table, [(0, 0)], positions, 0.125), BF16)
+    ops.check_status("cuda")
+
+
+@gpu
+def test_pools_of_more_than_31_bits_of_bytes(ops):
+    """Rows whose byte offsets need 32 bits and more: written, read back, attended to."""
+    pages, kv_heads, page, head_dim = 70_000, 8, 16, 128
+    codes = torch.zeros((pages, 2, kv_heads, page, head_dim), dtype=torch.int8, device="cuda")      # 2.3 GB
+    pool = ops.QuantizedPool(codes, torch.zeros(codes.shape[:4], device="cuda"))
+    assert codes.numel() > 1 << 31
+    held = [69_999, 69_000, 3, 66_123]
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn((60, kv_heads * head_dim), generator=gen, device="cuda").to(BF16) for _ in range(2))
+    ops.write_cache(k, v, pool, ints([held[t // 16] * 16 + t % 16 for t in range(60)]), ints(range(60)))
+    table = ints([held])
+    q = torch.randn((1, 16, head_dim), generator=gen, device="cuda").to(BF16)
+    out = torch.zeros_like(q)
+    ops.paged_attention_decode(q, pool, out, table, ints([0]), ints([0]), ints([59]), 0.1, 60)
+    small = ops.QuantizedPool(codes[held].contiguous(), pool.scales[held].contiguous())      # the same rows in a pool of four pages
+    order = ints([[0, 1, 2, 3]])
+    close(out, *exact_decode(q, small, order, [(0, 0)], ints([59]), 0.1), BF16)
+    back = torch.zeros(codes.shape, dtype=BF16, device="cuda")
+    ops.read_cache(pool, back, table, ints([0]), ints([59]), ints([59]))
+    expect = torch.zeros(small.shape, dtype=BF16, device="cuda")
+    ops.read_cache(small, expect, order, ints([0]), ints([59]), ints([59]))
+    assert torch.equal(back[held], expect) and back.count_nonzero() == expect.count_nonzero()
+    ops.check_status("cuda")
+    del back, codes, pool
+    torch.cuda.empty_cache()
+
+
+def _a_step(ops, kind, seed, tokens=5, heads=8, kv_heads=2, head_dim=128, page=16, width=40):
+    """A decode step's buffers: projections, pool, tables, lists; the call that stores, attends and reads back."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    pool = random_pool(ops, kind, tokens * width, kv_heads, page, head_dim, seed)
+    order = torch.randperm(tokens * width, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+    s = dict(pool=pool, table=order.view(tokens, width).cuda(), positions=ints([0] * tokens), slots=ints([0] * tokens),
+             qkv=torch.zeros((tokens, (heads + 2 * kv_heads) * head_dim), dtype=BF16, device="cuda"),
+             q=torch.zeros((tokens, heads, head_dim), dtype=BF16, device="cuda"),
+             out=torch.zeros((tokens, heads, head_dim), dtype=BF16, device="cuda"),
+             back=torch.zeros(pool.shape, dtype=BF16, device="cuda"), rows=ints(range(tokens)))
+    angle = torch.rand((page * width, head_dim // 2), generator=gen, device="cuda")
+    s["cos"], s["sin"] = angle.cos(), angle.sin()
+
+    def feed(turn):
+        """The next step's numbers, into the same buffers."""
+        g = torch.Generator(device="cuda").manual_seed(100 * seed + turn)
+        s["qkv"].copy_(torch.randn(s["qkv"].shape, generator=g, device="cuda"))
+        at = torch.randint(0, page * width, (tokens,), generator=g, device="cuda")
+        s["positions"].copy_(at)
+        s["slots"].copy_(s["table"].long().gather(1, (at // page)[:, None])[:, 0] * page + at % page)
+
+    def call():
+        hq, hk = heads * head_dim, kv_heads * head_dim
+        ops.qk_norm_rope_cache(s["qkv"][:, :hq], s["qkv"][:, hq:hq + hk], s["qkv"][:, hq + hk:], s["q"], pool, s["slots"], s["positions"],
+                               None, None, s["cos"], s["sin"], 0.0)
+        ops.paged_attention_decode(s["q"], pool, s["out"], s["table"], s["rows"], s["rows"], s["positions"], 0.09, page * width, settled=True)
+        ops.read_cache(pool, s["back"], s["table"], s["rows"], s["positions"], s["positions"])
+
+    def result():
+        return [t.clone() for t in (s["q"], s["out"], s["back"], pool.codes.view(torch.uint8), pool.scales)]
+    return feed, call, result
+
+
+@gpu
+@pytest.mark.parametrize("chained", [False, True])
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+def test_captured_steps_replay(ops, kind, chained):
+    """Two captured graphs of two steps of their own, replayed in turn with new numbers, with and without launches that
+    overlap: bit for bit what the calls themselves give."""
+    eager = [_a_step(ops, kind, seed) for seed in (1, 2)]
+    captured = [_a_step(ops, kind, seed) for seed in (1, 2)]
+    try:
+        ops.set_chained_launches(chained)
+        graphs = []
+        for feed, call, _ in captured:
+            feed(0)
+            call()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                call()
+            graphs.append(graph)
+        for feed, call, _ in eager:
+            feed(0)
+            call()
+        for turn in range(1, 6):
+            for one, other, graph in zip(eager, captured, graphs):
+                for feed, _, _ in (one, other):
+                    feed(turn)
+                one[1]()
+                graph.replay()
+        torch.cuda.synchronize()
+        for one, other in zip(eager, captured):
+            for a, b in zip(one[2](), other[2]()):
+                assert torch.equal(a, b)
+        ops.check_status("cuda")
+    finally:
+        ops.set_chained_launches(False)
+
+
+@gpu
+def test_steps_on_two_streams_at_once(ops):
+    alone = [_a_step(ops, "fp8", seed) for seed in (3, 4)]
+    beside = [_a_step(ops, "fp8", seed) for seed in (3, 4)]
+    streams = [torch.cuda.Stream() for _ in beside]
+    for feed, call, _ in alone:
+        for turn in range(20):
+            feed(turn)
+            call()
+    torch.cuda.synchronize()
+    for turn in range(20):
+        for (feed, call, _), stream in zip(beside, streams):
+            with torch.cuda.stream(stream):
+                feed(turn)
+                call()
+    torch.cuda.synchronize()
+    for one, other in zip(alone, beside):
+        for a, b in zip(one[2](), other[2]()):
+            assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("head_dim,heads,kv_heads", [(128, 8, 2), (256, 4, 2), (48, 4, 2)])
+def test_rows_written_right_ahead_are_seen(ops, head_dim, heads, kv_heads):
+    """With overlapping launches on, a write of whole contexts directly ahead of the attention: without ``settled`` it waits
+    for all of it."""
+    page, length, rows = 16, 1500, 6
+    pages, table = spread_tables([length] * rows, page, 2)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    at = torch.arange(length).repeat(rows)
+    slots = (table.cpu().long()[torch.arange(rows).repeat_interleave(length), at // page] * page + at % page).to(torch.int32).cuda()
+    q = torch.randn((rows, heads, head_dim), generator=gen, device="cuda").to(BF16)
+    positions = ints([length - 1] * rows)
+    try:
+        ops.set_chained_launches(True)
+        for turn in range(4):
+            pool = ops.QuantizedPool.zeros(pages, kv_heads, page, head_dim)
+            k, v = (torch.randn((rows * length, kv_heads * head_dim), generator=gen, device="cuda").to(BF16) for _ in range(2))
+            out = torch.zeros_like(q)
+            torch.cuda.synchronize()
+            ops.write_cache(k, v, pool, slots, at.to(torch.int32).cuda())
+            ops.paged_attention_decode(q, pool, out, table, ints(range(rows)), ints(range(rows)), positions, 0.1, length)
+            close(out, *exact_decode(q, pool, table, [(r, r) for r in range(rows)], positions, 0.1), BF16)
+    finally:
+        ops.set_chained_launches(False)
+    ops.check_status("cuda")
+
+
+@gpu
+def test_calls_of_nothing(ops):
+    pool = random_pool(ops, "fp8", 2, 2, 16, 64, 0)
+    none, q = ints([]), torch.zeros(0, 4, 64, dtype=BF16, device="cuda")
+    assert ops.paged_attention_decode(q, pool, q, ints([[0, 1]]), none, none, none, 0.1, 20) is q
+    before = pool.scales.clone()
+    empty = torch.zeros(0, 128, dtype=BF16, device="cuda")
+    ops.write_cache(empty, empty, pool, none, none)
+    out = torch.ones(pool.shape, device="cuda")
+    ops.read_cache(pool, out, ints([[0, 1]]), none, none, none)
+    ops.read_cache(pool, out, ints([[0, 1]]), ints([0]), ints([0]), ints([-1]))
+    assert out.eq(1).all() and torch.equal(pool.scales, before)
+    ops.check_status("cuda")
