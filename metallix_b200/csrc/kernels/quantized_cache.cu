@@ -312,6 +312,17 @@ template <typename T, int KIND> __device__ __forceinline__ void code_values(cons
   }
 }
 
+struct ReadArgs {
+  const uint8_t* codes;
+  const float* scales;
+  void* out;
+  const int* block_tables;
+  int max_pages;
+  const int *row_request, *first, *last;
+  int kv_heads, head_dim, page_tokens, num_pages, window, chunk, keep;
+  int* status;
+};
+
 // Pages back into the compute type, for rows of whole 16-byte pieces: a page's
 // codes are one run of memory, and so are its values, so a block takes
 // kReadPieces pieces of one page at a time, each thread all its loads in flight
@@ -322,26 +333,25 @@ constexpr int kReadBlocks = 8 * 148 * 8;   // of a launch, at most (or one a req
 
 template <typename T, int KIND>
 __global__ void __launch_bounds__(kReadThreads)
-read_cache_pieces_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out,
-                         const int* __restrict__ block_tables, int max_pages, const int* __restrict__ row_request,
-                         const int* __restrict__ first, const int* __restrict__ last, int kv_heads, int head_dim, int page_tokens,
-                         int num_pages, int window, int chunk, int keep, int* status) {
-  const int row = blockIdx.y, end = last[row];
+read_cache_pieces_kernel(const __grid_constant__ ReadArgs a) {
+  // No release ahead of the end: what follows may read `out` as a cache whose pages it takes to be settled.
+  chain_wait();   // the codes are the work of kernels ahead
+  const int row = blockIdx.y, end = a.last[row], head_dim = a.head_dim, page_tokens = a.page_tokens;
   if (end < 0) return;
-  const KeyWalk walk = key_walk(min(first_visible_key(max(first[row], 0), window, chunk), end), end, keep, page_tokens);
-  const int per_row = head_dim >> 4, rows = 2 * kv_heads * page_tokens, pieces = rows * per_row;
+  const KeyWalk walk = key_walk(min(first_visible_key(max(a.first[row], 0), a.window, a.chunk), end), end, a.keep, page_tokens);
+  const int per_row = head_dim >> 4, rows = 2 * a.kv_heads * page_tokens, pieces = rows * per_row;
   const int per_page = (pieces + kReadPieces - 1) / kReadPieces;
-  const int* table = block_tables + static_cast<size_t>(row_request[row]) * max_pages;
+  const int* table = a.block_tables + static_cast<size_t>(a.row_request[row]) * a.max_pages;
   for (int item = blockIdx.x; item < walk.count * per_page; item += gridDim.x) {
     const int step = item / per_page, slot = walk.tile(step), piece0 = (item - step * per_page) * kReadPieces;
-    const int page = slot < max_pages ? table[slot] : -1;
-    if (page < 0 || page >= num_pages) {
-      if (threadIdx.x == 0) atomicOr(status, kStatusBadPage);
+    const int page = slot < a.max_pages ? table[slot] : -1;
+    if (page < 0 || page >= a.num_pages) {
+      if (threadIdx.x == 0) atomicOr(a.status, kStatusBadPage);
       continue;
     }
     const int seen = end - slot * page_tokens + 1;   // rows of the page up to the last position
     const size_t base = static_cast<size_t>(page) * rows;
-    const uint4* src = reinterpret_cast<const uint4*>(codes + base * head_dim);
+    const uint4* src = reinterpret_cast<const uint4*>(a.codes + base * head_dim);
     uint4 held[kReadDepth];
     float scale[kReadDepth];
     bool there[kReadDepth];
@@ -350,9 +360,9 @@ read_cache_pieces_kernel(const uint8_t* __restrict__ codes, const float* __restr
       const int piece = piece0 + j * kReadThreads + threadIdx.x, line = piece / per_row;
       there[j] = piece < pieces && (seen >= page_tokens || line % page_tokens < seen);
       held[j] = there[j] ? src[piece] : make_uint4(0u, 0u, 0u, 0u);
-      scale[j] = there[j] ? scales[base + line] : 0.0f;
+      scale[j] = there[j] ? a.scales[base + line] : 0.0f;
     }
-    T* dst = out + base * head_dim;
+    T* dst = static_cast<T*>(a.out) + base * head_dim;
 #pragma unroll
     for (int j = 0; j < kReadDepth; ++j) {
       if (!there[j]) continue;
@@ -370,26 +380,24 @@ read_cache_pieces_kernel(const uint8_t* __restrict__ codes, const float* __restr
 // `out` stays as it is.
 template <typename T, int KIND>
 __global__ void __launch_bounds__(256)
-read_cache_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, T* __restrict__ out,
-                  const int* __restrict__ block_tables, int max_pages, const int* __restrict__ row_request,
-                  const int* __restrict__ first, const int* __restrict__ last, int kv_heads, int head_dim, int page_tokens,
-                  int num_pages, int window, int chunk, int keep, int* status) {
+read_cache_kernel(const __grid_constant__ ReadArgs a) {
+  chain_wait();
   const int slot = blockIdx.x, row = blockIdx.y;
-  const int begin = first_visible_key(max(first[row], 0), window, chunk), end = last[row];
-  const int key0 = slot * page_tokens;
-  if (key0 > end || (key0 + page_tokens <= begin && key0 >= keep)) return;
-  const int page = block_tables[static_cast<size_t>(row_request[row]) * max_pages + slot];
-  if (page < 0 || page >= num_pages) {
-    if (threadIdx.x == 0) atomicOr(status, kStatusBadPage);
+  const int begin = first_visible_key(max(a.first[row], 0), a.window, a.chunk), end = a.last[row];
+  const int key0 = slot * a.page_tokens;
+  if (key0 > end || (key0 + a.page_tokens <= begin && key0 >= a.keep)) return;
+  const int page = a.block_tables[static_cast<size_t>(a.row_request[row]) * a.max_pages + slot];
+  if (page < 0 || page >= a.num_pages) {
+    if (threadIdx.x == 0) atomicOr(a.status, kStatusBadPage);
     return;
   }
-  const int rows = min(page_tokens, end - key0 + 1);
-  const size_t base = static_cast<size_t>(page) * 2 * kv_heads * page_tokens;
-  for (int i = threadIdx.x; i < 2 * kv_heads * rows * head_dim; i += blockDim.x) {
-    const int line = i / head_dim, d = i - line * head_dim;
+  const int rows = min(a.page_tokens, end - key0 + 1);
+  const size_t base = static_cast<size_t>(page) * 2 * a.kv_heads * a.page_tokens;
+  for (int i = threadIdx.x; i < 2 * a.kv_heads * rows * a.head_dim; i += blockDim.x) {
+    const int line = i / a.head_dim, d = i - line * a.head_dim;
     const int head = line / rows, r = line - head * rows;
-    const size_t at = base + static_cast<size_t>(head) * page_tokens + r;
-    out[at * head_dim + d] = from_float<T>(code_value<KIND>(codes[at * head_dim + d]) * scales[at]);
+    const size_t at = base + static_cast<size_t>(head) * a.page_tokens + r;
+    static_cast<T*>(a.out)[at * a.head_dim + d] = from_float<T>(code_value<KIND>(a.codes[at * a.head_dim + d]) * a.scales[at]);
   }
 }
 
@@ -499,32 +507,20 @@ MXB_API int mxb_read_cache(const void* call, int bytes, cudaStream_t stream) {
   const int kind = static_cast<int>(c.kind), dtype = static_cast<int>(c.dtype), rows = static_cast<int>(c.rows),
             kv_heads = static_cast<int>(c.kv_heads), head_dim = static_cast<int>(c.head_dim), max_pages = static_cast<int>(c.max_pages),
             page_tokens = static_cast<int>(c.page_tokens), num_pages = static_cast<int>(c.num_pages);
-  void* out = c.out;
   if (rows > 65535 || !pool_fits(num_pages, kv_heads, page_tokens) || head_dim <= 0 || head_dim > 512 ||
       (dtype != kF32 && dtype != kBF16) || (kind != kCodesE4M3 && kind != kCodesInt8))
     return static_cast<int>(cudaErrorInvalidValue);
-  const bool by_pieces = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(c.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const bool by_pieces = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(c.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(c.out) % 16 == 0;
   // A block an item where tables are short; wide tables of short contexts (a captured step's) walk with a stride instead.
   const long long items = static_cast<long long>(max_pages) * ((2LL * kv_heads * page_tokens * (head_dim / 16) + kReadPieces - 1) / kReadPieces);
   const long long most = kReadBlocks / rows > 0 ? kReadBlocks / rows : 1;
   const dim3 grid(static_cast<unsigned>(!by_pieces ? max_pages : (items < most ? items : most)), rows);
-  auto launch = [&](auto kernel, auto* target) {
-    kernel<<<grid, kReadThreads, 0, stream>>>(static_cast<const uint8_t*>(c.codes), c.scales, target, c.block_tables,
-                                                     max_pages, c.row_request, c.first, c.last, kv_heads, head_dim, page_tokens,
-                                                     num_pages, static_cast<int>(c.window), static_cast<int>(c.chunk),
-                                                     static_cast<int>(c.keep), c.status);
-    return static_cast<int>(cudaGetLastError());
-  };
-  if (by_pieces) {
-    if (dtype == kF32)
-      return kind == kCodesInt8 ? launch(read_cache_pieces_kernel<float, kCodesInt8>, static_cast<float*>(out))
-                                : launch(read_cache_pieces_kernel<float, kCodesE4M3>, static_cast<float*>(out));
-    return kind == kCodesInt8 ? launch(read_cache_pieces_kernel<__nv_bfloat16, kCodesInt8>, static_cast<__nv_bfloat16*>(out))
-                              : launch(read_cache_pieces_kernel<__nv_bfloat16, kCodesE4M3>, static_cast<__nv_bfloat16*>(out));
-  }
-  if (dtype == kF32)
-    return kind == kCodesInt8 ? launch(read_cache_kernel<float, kCodesInt8>, static_cast<float*>(out))
-                              : launch(read_cache_kernel<float, kCodesE4M3>, static_cast<float*>(out));
-  return kind == kCodesInt8 ? launch(read_cache_kernel<__nv_bfloat16, kCodesInt8>, static_cast<__nv_bfloat16*>(out))
-                            : launch(read_cache_kernel<__nv_bfloat16, kCodesE4M3>, static_cast<__nv_bfloat16*>(out));
+  const ReadArgs args = {static_cast<const uint8_t*>(c.codes), c.scales, c.out, c.block_tables, max_pages, c.row_request, c.first, c.last,
+                         kv_heads, head_dim, page_tokens, num_pages, static_cast<int>(c.window), static_cast<int>(c.chunk),
+                         static_cast<int>(c.keep), c.status};
+  auto launch = [&](auto kernel) { return static_cast<int>(launch_chained(kernel, grid, dim3(kReadThreads), 0, stream, args)); };
+#define BY_TYPE(KERNEL) (dtype == kF32 ? (kind == kCodesInt8 ? launch(KERNEL<float, kCodesInt8>) : launch(KERNEL<float, kCodesE4M3>)) \
+                                       : (kind == kCodesInt8 ? launch(KERNEL<__nv_bfloat16, kCodesInt8>) : launch(KERNEL<__nv_bfloat16, kCodesE4M3>)))
+  return by_pieces ? BY_TYPE(read_cache_pieces_kernel) : BY_TYPE(read_cache_kernel);
+#undef BY_TYPE
 }

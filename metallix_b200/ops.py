@@ -1326,14 +1326,16 @@ class QuantizedPool:
     compute type; ``read_cache`` turns pages back into such a cache, which the
     other attention kernels read."""
 
-    __slots__ = ("codes", "scales")
+    __slots__ = ("codes", "scales", "shape", "device_index", "kind")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         self.codes, self.scales = codes, scales
-        if not (type(codes) is type(scales) is torch.Tensor and codes.dtype in _CODE_KINDS and scales.dtype is torch.float32
-                and codes.is_contiguous() and scales.is_contiguous() and codes.dim() == 5 and codes.shape[1] == 2
-                and scales.shape == codes.shape[:4] and codes.is_cuda and codes.get_device() == scales.get_device()
-                and scales.numel() < 1 << 31):
+        if not isinstance(codes, torch.Tensor):
+            self._refuse()
+        self.shape, self.device_index, self.kind = shape, device, _ = codes.shape, codes.get_device(), _CODE_KINDS.get(codes.dtype)
+        if not (self.kind is not None and device >= 0 and len(shape) == 5 and shape[1] == 2 and codes.is_contiguous()
+                and isinstance(scales, torch.Tensor) and scales.dtype is torch.float32 and scales.shape == shape[:4]
+                and scales.is_contiguous() and scales.get_device() == device and scales.numel() < 1 << 31):
             self._refuse()
 
     def _refuse(self) -> None:
@@ -1352,14 +1354,6 @@ class QuantizedPool:
         shape = (pages, 2, kv_heads, page_tokens, head_dim)
         return cls(torch.zeros(shape, dtype=CODE_DTYPES[codes], device=device),
                    torch.zeros(shape[:4], dtype=torch.float32, device=device))
-
-    @property
-    def shape(self) -> torch.Size:
-        return self.codes.shape
-
-    @property
-    def kind(self) -> int:
-        return _CODE_KINDS[self.codes.dtype]
 
 
 def _on_current_device(*tensors) -> None:
@@ -1395,8 +1389,7 @@ def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tenso
     block tables serve it; rows that are not read stay as they are. A negative
     ``last`` reads nothing."""
     _need(isinstance(pool, QuantizedPool), "pool must be a QuantizedPool")
-    codes = pool.codes
-    shape, device = codes.shape, codes.get_device()
+    codes, shape, device = pool.codes, pool.shape, pool.device_index
     rows = row_request.numel() if isinstance(row_request, torch.Tensor) else 0
     if not (isinstance(out, torch.Tensor) and out.dtype in _CODES and out.shape == shape and out.is_contiguous()
             and out.get_device() == device == _current_device() and _ints_on(device, 2, block_tables)
@@ -1411,11 +1404,11 @@ def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tenso
         _need(rows <= 65535, f"{rows} rows in one call; up to 65535")
         _need(shape[4] <= 512, f"head_dim {shape[4]} is beyond 512")
         _on_current_device(codes, out, block_tables, row_request, first, last)
-    if rows and codes.numel():
+    if rows and 0 not in shape:
         num_pages, _, kv_heads, page_tokens, head_dim = shape
         call = _READ_CALL.pack(
             codes.data_ptr(), pool.scales.data_ptr(), out.data_ptr(), block_tables.data_ptr(), row_request.data_ptr(),
-            first.data_ptr(), last.data_ptr(), _status_pointer(device), _CODE_KINDS[codes.dtype], _CODES[out.dtype],
+            first.data_ptr(), last.data_ptr(), _status_pointer(device), pool.kind, _CODES[out.dtype],
             block_tables.shape[1], rows, kv_heads, head_dim, page_tokens, num_pages, window or 0, chunk or 0,
             _kept(keep) if keep else 0)
         _call("mxb_read_cache", call, len(call), _stream())
@@ -1497,14 +1490,13 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
 def _store_quantized(q, k, v, q_out, pool: QuantizedPool, slots, positions, q_weight, k_weight, cos, sin, eps: float,
                      interleaved: bool, norm_scope: str, q_factors) -> None:
     """``qk_norm_rope_cache`` into a quantized pool."""
-    codes, dtype = pool.codes, q.dtype
-    device = codes.get_device()
-    num_pages, _, kv_heads, page_tokens, head_dim = codes.shape
-    for tensor in (q, k, v):
-        if not (tensor.dtype is dtype and tensor.dim() == 2 and tensor.stride(1) == 1 and tensor.get_device() == device
-                and dtype in _CODES):
-            raise KernelError("q, k and v must be CUDA [tokens, width] tensors with unit column stride, of one type and on the "
-                              "pool's device")
+    dtype, device = q.dtype, pool.device_index
+    num_pages, _, kv_heads, page_tokens, head_dim = pool.shape
+    q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
+    if not (dtype is k.dtype is v.dtype and dtype in _CODES and len(q_stride) == len(k_stride) == len(v_stride) == 2
+            and q_stride[1] == k_stride[1] == v_stride[1] == 1 and q.get_device() == k.get_device() == v.get_device() == device):
+        raise KernelError("q, k and v must be CUDA [tokens, width] tensors with unit column stride, of one type and on the "
+                          "pool's device")
     tokens, width = q.shape
     heads = width // head_dim
     if not (width == heads * head_dim and k.shape == v.shape == (tokens, kv_heads * head_dim)):
@@ -1515,7 +1507,7 @@ def _store_quantized(q, k, v, q_out, pool: QuantizedPool, slots, positions, q_we
         _check(slots, "slots", (torch.int32,), 1)
         _need(positions.numel() == tokens, "token counts differ")
         _need(slots.numel() == tokens, "one slot per token")
-        _on_current_device(codes, slots, positions)
+        _on_current_device(pool.codes, slots, positions)
     _need(head_dim <= 512 and heads + 2 * kv_heads <= 65535, "heads of up to 512 values, up to 65535 of them")
     if q_out is not None and not (q_out.dtype is dtype and q_out.is_contiguous() and q_out.shape == (tokens, heads, head_dim)
                                   and q_out.get_device() == device):
@@ -1547,10 +1539,11 @@ def _store_quantized(q, k, v, q_out, pool: QuantizedPool, slots, positions, q_we
         factors = q_factors.numel()
     sums = torch.empty(2 * tokens, dtype=torch.float32, device=q.device) if projection else None
     call = _STORE_CALL.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(q_out) or 0, codes.data_ptr(), pool.scales.data_ptr(),
-        slots.data_ptr(), positions.data_ptr(), _ptr(q_weight) or 0, _ptr(k_weight) or 0, _ptr(cos) or 0, _ptr(sin) or 0,
-        _ptr(sums) or 0, _ptr(q_factors) or 0, _status_pointer(device), q.stride(0), k.stride(0), v.stride(0),
-        _CODE_KINDS[codes.dtype], _CODES[dtype], table_positions, rotary_dim, 1 if interleaved else 0, 1 if projection else 0,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q_out is None else q_out.data_ptr(), pool.codes.data_ptr(),
+        pool.scales.data_ptr(), slots.data_ptr(), positions.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(),
+        0 if k_weight is None else k_weight.data_ptr(), 0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(),
+        0 if sums is None else sums.data_ptr(), 0 if q_factors is None else q_factors.data_ptr(), _status_pointer(device),
+        q_stride[0], k_stride[0], v_stride[0], pool.kind, _CODES[dtype], table_positions, rotary_dim, 1 if interleaved else 0, 1 if projection else 0,
         tokens, heads, kv_heads, head_dim, page_tokens, num_pages, factors, eps)
     _call("mxb_store_quantized", call, len(call), _stream())
 
@@ -1816,9 +1809,8 @@ def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.
     """The decode attention over a quantized pool, into ``out`` or, with the
     output projection ``weight``, into ``summands``."""
     global _split_keys
-    codes, dtype = pool.codes, q.dtype
-    device = codes.get_device()
-    num_pages, _, kv_heads, page_tokens, cache_dim = codes.shape
+    codes, dtype, device = pool.codes, q.dtype, pool.device_index
+    num_pages, _, kv_heads, page_tokens, cache_dim = pool.shape
     if not (q.dim() == 3 and dtype in _CODES and q.is_contiguous() and q.get_device() == device == _current_device()
             and (out is None or (out.dtype is dtype and out.shape == q.shape and out.is_contiguous() and out.get_device() == device))):
         _check(q, "q", _COMPUTE, 3)
@@ -1863,9 +1855,10 @@ def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.
     if not rows:
         return
     fields = [
-        q.data_ptr(), codes.data_ptr(), pool.scales.data_ptr(), _ptr(out) or 0, _ptr(partial) or 0, block_tables.data_ptr(),
-        row_token.data_ptr(), row_request.data_ptr(), positions.data_ptr(), _ptr(weight) or 0, _ptr(summands) or 0, _ptr(gate) or 0,
-        sink_heads or 0, bias_table or 0, _status_pointer(device), _CODE_KINDS[codes.dtype], _CODES[dtype],
+        q.data_ptr(), codes.data_ptr(), pool.scales.data_ptr(), 0 if out is None else out.data_ptr(),
+        0 if partial is None else partial.data_ptr(), block_tables.data_ptr(), row_token.data_ptr(), row_request.data_ptr(),
+        positions.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if summands is None else summands.data_ptr(),
+        0 if gate is None else gate.data_ptr(), sink_heads or 0, bias_table or 0, _status_pointer(device), pool.kind, _CODES[dtype],
         block_tables.shape[1], rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits, window or 0, chunk or 0,
         _kept(keep) if keep else 0, ldw, hidden, gate_stride, has_sink, bias_far, 1 if settled else 0, scale, softcap, sink_score]
     call, stream = _QUANTIZED_DECODE_CALL.pack(*fields), _stream()

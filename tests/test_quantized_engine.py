@@ -97,8 +97,8 @@ def test_single_tokens_over_codes_need_their_kernel():
     from metallix_b200.parts.attention import attend_cached
     from metallix_b200.parts.registry import CacheView
 
-    pool = object.__new__(ops.QuantizedPool)
-    pool.codes, pool.scales = torch.zeros(3, 2, 1, 4, 8, dtype=torch.int8), torch.zeros(3, 2, 1, 4)
+    pool = object.__new__(ops.QuantizedPool)     # as if on a device
+    pool.shape = torch.Size((3, 2, 1, 4, 8))
 
     class Context:
         extras = {"attention_tiles": {"multi_tiles": 0, "decode_rows": 1, "read_request": torch.zeros(0)}}
