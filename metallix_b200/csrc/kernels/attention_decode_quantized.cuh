@@ -432,6 +432,7 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
 #pragma unroll
   for (int i = 0; i < HD / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
   int given_up_at = stages;
+  bool begun = false;   // whether a stage has set the reference
 
   for (int i = 0; i < stages; ++i) {
     const int slot = i % STAGES;
@@ -455,9 +456,11 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
     // ---- scores: eight b, this lane has key b * 8 + g and heads 2t, 2t + 1
     float s[EIGHTS][2];
     {
-      float d[EIGHTS / 2][4];
+      float d[2][EIGHTS / 2][4];   // two sums each, so that a product waits for half as many
 #pragma unroll
-      for (int h = 0; h < EIGHTS / 2; ++h) d[h][0] = d[h][1] = d[h][2] = d[h][3] = 0.0f;
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int h = 0; h < EIGHTS / 2; ++h) d[x][h][0] = d[x][h][1] = d[x][h][2] = d[x][h][3] = 0.0f;
 #pragma unroll
       for (int j = 0; j < Tile::kChunks; ++j) {
         uint32_t words[EIGHTS][4];
@@ -473,15 +476,15 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
             code_halves<KIND>(words[2 * h][w], a0, a2);
             code_halves<KIND>(words[2 * h + 1][w], a1, a3);
 #pragma unroll
-            for (int x = 0; x < PARTS; ++x) quant_mma(d[h], a0, a1, a2, a3, q0[n][x], q2[n][x]);
+            for (int x = 0; x < PARTS; ++x) quant_mma(d[(PARTS == 2 ? x : w) & 1][h], a0, a1, a2, a3, q0[n][x], q2[n][x]);
           }
         }
       }
 #pragma unroll
       for (int b = 0; b < EIGHTS; ++b) {
         const float k_scale = scales[b * 8 + g];
-        s[b][0] = d[b / 2][2 * (b & 1)] * to_score[0] * k_scale;
-        s[b][1] = d[b / 2][2 * (b & 1) + 1] * to_score[1] * k_scale;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s[b][j] = (d[0][b / 2][2 * (b & 1) + j] + d[1][b / 2][2 * (b & 1) + j]) * to_score[j] * k_scale;
       }
     }
     if (scaled) {
@@ -501,7 +504,20 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
     }
     float weight[EIGHTS][2];
     float sum[2], widest[2];
-    auto weigh = [&]() {
+    for (bool anew = !begun;; anew = true) {   // once more where the weights outgrew their room: with a new reference
+      float carry[2] = {1.0f, 1.0f};
+      if (anew) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float most = m[j];
+#pragma unroll
+          for (int b = 0; b < EIGHTS; ++b) most = fmaxf(most, s[b][j]);
+#pragma unroll
+          for (int offset = 4; offset < 32; offset <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
+          carry[j] = quant_exp2<T>(m[j] - most);   // what was gathered so far, on the new reference
+          m[j] = most;
+        }
+      }
       sum[0] = sum[1] = widest[0] = widest[1] = 0.0f;
 #pragma unroll
       for (int b = 0; b < EIGHTS; ++b) {
@@ -514,22 +530,11 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
           widest[j] = fmaxf(widest[j], weight[b][j]);
         }
       }
-    };
-    weigh();
-    const bool outgrown = fmaxf(sum[0], sum[1]) > 65536.0f || fmaxf(widest[0] * up[0], widest[1] * up[1]) >= 32768.0f;
-    if (__any_sync(0xffffffffu, outgrown)) {
-      float carry[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float most = m[j];
-#pragma unroll
-        for (int b = 0; b < EIGHTS; ++b) most = fmaxf(most, s[b][j]);
-#pragma unroll
-        for (int offset = 4; offset < 32; offset <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
-        carry[j] = quant_exp2<T>(m[j] - most);   // what was gathered so far, on the new reference
-        m[j] = most;
+      if (!anew) {
+        const bool outgrown = fmaxf(sum[0], sum[1]) > 65536.0f || fmaxf(widest[0] * up[0], widest[1] * up[1]) >= 32768.0f;
+        if (!__any_sync(0xffffffffu, outgrown)) break;
+        continue;
       }
-      weigh();
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float most = widest[j];
@@ -541,9 +546,13 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
         // a quotient beyond float32 means that what was gathered is nothing on the new reference: carry is 0 then
         const float factor = carry[j] * fminf(up[j] / before, 0x1p127f);
         l[j] *= carry[j];
+        if (begun) {
 #pragma unroll
-        for (int n = 0; n < HD / 16; ++n) { o[n][j] *= factor; o[n][2 + j] *= factor; }
+          for (int n = 0; n < HD / 16; ++n) { o[n][j] *= factor; o[n][2 + j] *= factor; }
+        }
       }
+      begun = true;
+      break;
     }
     l[0] += sum[0];
     l[1] += sum[1];
@@ -606,7 +615,7 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
   __syncthreads();
   float* merge = reinterpret_cast<float*>(quant_shared);   // [warps][8 heads][HD + 2]
   {
-    const float d0 = 1.0f / up[0], d1 = 1.0f / up[1];   // powers of two
+    const float d0 = __fdividef(1.0f, up[0]), d1 = __fdividef(1.0f, up[1]);   // powers of two
 #pragma unroll
     for (int n = 0; n < HD / 16; ++n) {
       constexpr int BLOCKS = Tile::kValueBytes / 2;   // of 16 values, from one piece
@@ -659,7 +668,7 @@ static int quantized_slots(int pairs, int tiles, int resident) {
   const int twice = pairs <= resident ? 2 * resident / pairs : (2 * resident + pairs / 2) / pairs;
   if (pairs > 1 && twice > 1 && tiles >= 8 * twice) return twice;
   int slots = resident / pairs;
-  const int most = tiles <= 8 ? tiles : (tiles / 2 > 8 ? tiles / 2 : 8);
+  const int most = tiles <= 16 ? tiles : (tiles / 2 > 16 ? tiles / 2 : 16);
   if (slots > most) slots = most;
   return slots > 1 ? slots : 1;
 }

@@ -64,7 +64,7 @@ template <int KIND> __device__ __forceinline__ RowScale row_scale(uint32_t large
   r.scale = __fdiv_rn(__uint_as_float(largest), CodeLimit<KIND>::value);
   r.shift = r.scale < 0x1p-60f ? 0x1p80f : (r.scale > 0x1p60f ? 0x1p-80f : 1.0f);
   r.divisor = r.scale * r.shift;   // exact
-  r.inverse = r.divisor > 0.0f ? __fdiv_rn(1.0f, r.divisor) : 0.0f;
+  r.inverse = r.divisor > 0.0f ? __frcp_rn(r.divisor) : 0.0f;
   return r;
 }
 

@@ -524,3 +524,5 @@ MXB_API int mxb_read_cache(const void* call, int bytes, cudaStream_t stream) {
   return by_pieces ? BY_TYPE(read_cache_pieces_kernel) : BY_TYPE(read_cache_kernel);
 #undef BY_TYPE
 }
+
+MXB_TIMELINE_EXPORT(mxb_timeline_quantized_cache)
