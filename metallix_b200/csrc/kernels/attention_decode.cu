@@ -1349,7 +1349,7 @@ MXB_API int mxb_paged_attention_decode_quantized(const void* call, int bytes, cu
                                 static_cast<int>(c.max_pages), c.row_token, c.row_request, c.positions, heads, kv_heads, head_dim,
                                 static_cast<int>(c.page_tokens), static_cast<int>(c.num_pages), window, chunk, keep,
                                 static_cast<float>(c.scale), static_cast<float>(c.softcap),
-                                ScoreBias{c.bias_table, static_cast<int>(c.bias_far)}, page_shift, static_cast<int>(c.settled), c.status,
+                                ScoreBias{c.bias_table, static_cast<int>(c.bias_far)}, heads / kv_heads, page_shift, static_cast<int>(c.settled), c.status,
                                 0, max_splits, c.out, c.gate, c.gate_stride, has_sink, sink_score, c.sink_heads};
   int slots = 1;
   const cudaError_t e = dtype == kF32 ? launch_quantized_decode<float>(args, kind, rows, c.w == nullptr, &slots, stream)

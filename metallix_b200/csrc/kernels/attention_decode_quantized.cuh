@@ -26,6 +26,7 @@ struct QuantizedDecode {
   int heads, kv_heads, head_dim, page_tokens, num_pages, window, chunk, keep;
   float scale, softcap;
   ScoreBias bias;
+  int group;                     // query heads a key/value head
   int page_shift;                // log2 of page_tokens, -1 where that is no power of two
   int settled;                   // the positions ahead of each token's own were written by launches before the last one
   int* status;
@@ -267,24 +268,33 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
   unsigned char* quant_shared = quant_raw + ((1024 - (shared_address(quant_raw) & 1023)) & 1023);
   const bool release_late = gridDim.x * gridDim.y * gridDim.z > QuantBlocks<T, HD>::value * 148u;   // as in the kernels over bfloat16 rows
   if (!release_late) chain_release();
-  const int rank = blockIdx.x, slots = gridDim.x, kv = blockIdx.y % a.kv_heads, part = blockIdx.y / a.kv_heads, row = blockIdx.z;
+  const int rank = blockIdx.x, slots = gridDim.x, row = blockIdx.z, group = a.group;
+  int kv = blockIdx.y, part = 0;   // key/value head, and which eight of its query heads
+  for (; kv >= a.kv_heads; kv -= a.kv_heads) ++part;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   // Pages are a power of two of 8 positions or more: a box is a page's rows of one plane, or of a stage where a page has more.
   // Lane n has box n fetched (keys' boxes, then values'; for heads of 256 each as two halves) and looks after key n's scales.
   // Pages are asked for one stage ahead of the copies, and looked at only then; those of the first stage together with the
   // position, on the guess that neither a window nor a chunk has moved the first tile.
-  constexpr int WIDE = HD / Tile::kBoxBytes;   // boxes a row is cut into
-  const int shift = a.page_shift, in_page = a.page_tokens - 1, box_keys = min(a.page_tokens, KEYS);
-  const int per_plane = KEYS / box_keys, boxes = 2 * per_plane * WIDE;
-  const int plane = lane / (per_plane * WIDE), box = lane % (per_plane * WIDE) / WIDE, wide = lane % WIDE;
-  const int box_key = box * box_keys, scale_key = lane % KEYS;
+  constexpr int WIDE = HD / Tile::kBoxBytes, KEYS_LOG = KEYS == 32 ? 5 : 4, WIDE_LOG = WIDE - 1;   // WIDE boxes a row is cut into: 1 or 2
+  const int shift = a.page_shift, in_page = a.page_tokens - 1, box_shift = min(shift, KEYS_LOG), box_keys = 1 << box_shift;
+  const int plane_log = KEYS_LOG - box_shift + WIDE_LOG, boxes = 2 << plane_log;   // boxes of a plane, as a power of two
+  const int plane = lane >> plane_log, box = (lane & ((1 << plane_log) - 1)) >> WIDE_LOG, wide = lane & (WIDE - 1);
+  const int box_key = box << box_shift, scale_key = lane % KEYS;
   if (!a.settled) chain_wait();
-  const int token = a.row_token[row];
-  const int* table = a.block_tables + static_cast<size_t>(a.row_request[row]) * a.max_pages;
+  const int token = a.row_token[row], request = a.row_request[row];
+  uint64_t* landed = barriers + warp * STAGES;
+  if (lane == 0) {   // while those are on their way
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) barrier_init(&landed[i], 1);
+    barrier_init_fence();
+  }
+  __syncwarp();
+  const int* table = a.block_tables + static_cast<size_t>(request) * a.max_pages;
   auto page_at = [&](int key) { return (key >> shift) < a.max_pages ? table[key >> shift] : -1; };
   int box_page = page_at(rank * kSplitKeys + warp * 32 + box_key), scale_page = page_at(rank * kSplitKeys + warp * 32 + scale_key);
   if (token < 0) return;   // a padding row
-  const int pos = a.positions[token], group = a.heads / a.kv_heads;
+  const int pos = a.positions[token];
   const int live = min(group - part * 8, 8), head0 = kv * group + part * 8;   // this block's query heads
   const int first_key = first_visible_key(pos, a.window, a.chunk);
   const KeyWalk walk = key_walk(first_key, pos, a.keep, kSplitKeys);
@@ -328,13 +338,6 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
   }
   unsigned char* ring = quant_shared + warp * Tile::kWarpBytes;
   float* ring_scales = reinterpret_cast<float*>(quant_shared + WARPS * Tile::kWarpBytes) + warp * (STAGES * Tile::kScales);
-  uint64_t* landed = barriers + warp * STAGES;
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < STAGES; ++i) barrier_init(&landed[i], 1);
-    barrier_init_fence();
-  }
-  __syncwarp();
 
   // Stage i of the warp: part i % HALVES of its keys of the block's tile i / HALVES.
   const int stages = HALVES * ((walk.count - rank + slots - 1) / slots);
@@ -352,13 +355,13 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
       if (lane == 0) barrier_arrive_expect(&landed[slot], 2 * Tile::kRowBytes);
       __syncwarp();
       if (lane < boxes) {
-        const int key = key0 + box * box_keys;
+        const int key = key0 + box_key;
         bool there = wanted(key, box_keys);
         if (there && (box_page < 0 || box_page >= a.num_pages)) {
           atomicOr(a.status, kStatusBadPage);
           there = false;
         }
-        tma_load_2d(ring + slot * (2 * Tile::kRowBytes) + plane * Tile::kRowBytes + wide * (KEYS * 128) + box * box_keys * Tile::kBoxBytes,
+        tma_load_2d(ring + slot * (2 * Tile::kRowBytes) + plane * Tile::kRowBytes + wide * (KEYS * 128) + box_key * Tile::kBoxBytes,
                     &map_codes, wide * Tile::kBoxBytes,
                     there ? row_in(box_page, key) + plane * value_rows : a.num_pages * 2 * value_rows, &landed[slot]);
       }
