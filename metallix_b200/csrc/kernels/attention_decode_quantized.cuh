@@ -153,9 +153,9 @@ quantized_decode_kernel(const QuantizedDecode a) {
 // A warp works alone until the end: it takes its 32 keys of a 128-key tile (a
 // stage; for heads of 256, 16 of them) and has their rows brought into a ring of
 // its own by TMA, one box per page and plane with the swizzle that lets its lanes
-// read them without bank conflicts. (Copies of 16 bytes a lane by cp.async kept
-// an SM to 34 GB/s times its clock's share however many were under way and
-// however little else was done: 122 us for 8 requests over 32,000 positions.)
+// read them without bank conflicts. (With copies of 16 bytes a lane by cp.async
+// 8 requests over 32,000 positions took 113 to 130 us, whatever depth and number
+// of blocks an SM was tried; by TMA 87.6 when they were changed.)
 // What a lane reads is chosen so that bytes need no transposing:
 //   K: lane (g, t) = (lane / 4, lane % 4) reads the 16-byte chunks 2t, 2t + 1 of the
 //      key g of eight (heads of 64: chunk t). Word w of a chunk of the keys g and
