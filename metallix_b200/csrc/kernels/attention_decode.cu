@@ -1338,7 +1338,7 @@ MXB_API int mxb_paged_attention_decode_quantized(const void* call, int bytes, cu
   const float sink_score = static_cast<float>(c.sink_score);
   if (!quantized_decode_takes(head_dim, heads, kv_heads, dtype) || max_splits <= 0 || c.page_tokens <= 0 ||
       c.num_pages <= 0 || rows > 65535 || (kind != kCodesE4M3 && kind != kCodesInt8) || (c.bias_table != nullptr && c.bias_far < 0) ||
-      c.num_pages * 2 * kv_heads * c.page_tokens > 0x7fffffffLL)
+      c.num_pages * 2 * kv_heads * c.page_tokens > 0x7fffffffLL || static_cast<long long>(rows) * heads > 0x7fffffffLL)
     return static_cast<int>(cudaErrorInvalidValue);
   if (c.w != nullptr && (dtype != kBF16 || hidden <= 0 || !decode_project_takes(head_dim, tokens, c.w, c.ldw)))
     return static_cast<int>(cudaErrorInvalidValue);

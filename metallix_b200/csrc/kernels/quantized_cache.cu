@@ -508,6 +508,7 @@ MXB_API int mxb_read_cache(const void* call, int bytes, cudaStream_t stream) {
             kv_heads = static_cast<int>(c.kv_heads), head_dim = static_cast<int>(c.head_dim), max_pages = static_cast<int>(c.max_pages),
             page_tokens = static_cast<int>(c.page_tokens), num_pages = static_cast<int>(c.num_pages);
   if (rows > 65535 || !pool_fits(num_pages, kv_heads, page_tokens) || head_dim <= 0 || head_dim > 512 ||
+      2LL * kv_heads * page_tokens * head_dim > 0x7fffffffLL ||   // a page's codes are counted in 31 bits
       (dtype != kF32 && dtype != kBF16) || (kind != kCodesE4M3 && kind != kCodesInt8))
     return static_cast<int>(cudaErrorInvalidValue);
   const bool by_pieces = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(c.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(c.out) % 16 == 0;

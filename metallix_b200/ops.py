@@ -1356,6 +1356,15 @@ class QuantizedPool:
                    torch.zeros(shape[:4], dtype=torch.float32, device=device))
 
 
+_FAR = 1 << 30   # positions that a pool of 31 bits of rows can hold: windows and chunks of that many limit nothing
+
+
+def _reach(value) -> int:
+    """A window or chunk as the kernels over codes take it, in 31 bits (0: none)."""
+    value = int(value or 0)
+    return value if value < _FAR else 0
+
+
 def _on_current_device(*tensors) -> None:
     """The kernels run on the current device's current stream: everything has to be there."""
     current = _current_device()
@@ -1409,8 +1418,8 @@ def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tenso
         call = _READ_CALL.pack(
             codes.data_ptr(), pool.scales.data_ptr(), out.data_ptr(), block_tables.data_ptr(), row_request.data_ptr(),
             first.data_ptr(), last.data_ptr(), _status_pointer(device), pool.kind, _CODES[out.dtype],
-            block_tables.shape[1], rows, kv_heads, head_dim, page_tokens, num_pages, window or 0, chunk or 0,
-            _kept(keep) if keep else 0)
+            block_tables.shape[1], rows, kv_heads, head_dim, page_tokens, num_pages, _reach(window), _reach(chunk),
+            min(_kept(keep), _FAR) if keep else 0)
         _call("mxb_read_cache", call, len(call), _stream())
     return out
 
@@ -1429,8 +1438,9 @@ def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_out:
     (i, i + rotary_dim / 2), or (2i, 2i + 1) when ``interleaved``), q written to ``q_out``
     [tokens, heads, head_dim], k and v written into ``cache``
     [pages, 2, kv_heads, page_tokens, head_dim] at ``slots`` (a negative slot
-    skips the token; ``cache=None`` writes nothing; a ``QuantizedPool`` takes
-    the rows, unrounded, as codes and scales). q, k and v are
+    skips the token, two tokens of a call may not have the same one;
+    ``cache=None`` writes nothing; a ``QuantizedPool`` takes the rows, unrounded,
+    as codes and scales). q, k and v are
     [tokens, heads * head_dim] views whose rows may be strided. ``q_factors``
     (float32, one per position): what the queries are multiplied by."""
     if isinstance(cache, QuantizedPool):
@@ -1492,6 +1502,7 @@ def _store_quantized(q, k, v, q_out, pool: QuantizedPool, slots, positions, q_we
     """``qk_norm_rope_cache`` into a quantized pool."""
     dtype, device = q.dtype, pool.device_index
     num_pages, _, kv_heads, page_tokens, head_dim = pool.shape
+    _need(0 < head_dim <= 512, f"head_dim {head_dim} is not between 1 and 512")
     q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
     if not (dtype is k.dtype is v.dtype and dtype in _CODES and len(q_stride) == len(k_stride) == len(v_stride) == 2
             and q_stride[1] == k_stride[1] == v_stride[1] == 1 and q.get_device() == k.get_device() == v.get_device() == device):
@@ -1508,7 +1519,7 @@ def _store_quantized(q, k, v, q_out, pool: QuantizedPool, slots, positions, q_we
         _need(positions.numel() == tokens, "token counts differ")
         _need(slots.numel() == tokens, "one slot per token")
         _on_current_device(pool.codes, slots, positions)
-    _need(head_dim <= 512 and heads + 2 * kv_heads <= 65535, "heads of up to 512 values, up to 65535 of them")
+    _need(heads + 2 * kv_heads <= 65535, "up to 65535 heads")
     if q_out is not None and not (q_out.dtype is dtype and q_out.is_contiguous() and q_out.shape == (tokens, heads, head_dim)
                                   and q_out.get_device() == device):
         _check(q_out, "q_out", (dtype,), 3)
@@ -1859,8 +1870,8 @@ def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.
         0 if partial is None else partial.data_ptr(), block_tables.data_ptr(), row_token.data_ptr(), row_request.data_ptr(),
         positions.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if summands is None else summands.data_ptr(),
         0 if gate is None else gate.data_ptr(), sink_heads or 0, bias_table or 0, _status_pointer(device), pool.kind, _CODES[dtype],
-        block_tables.shape[1], rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits, window or 0, chunk or 0,
-        _kept(keep) if keep else 0, ldw, hidden, gate_stride, has_sink, bias_far, 1 if settled else 0, scale, softcap, sink_score]
+        block_tables.shape[1], rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits, _reach(window),
+        _reach(chunk), min(_kept(keep), _FAR) if keep else 0, ldw, hidden, gate_stride, has_sink, bias_far, 1 if settled else 0, scale, softcap, sink_score]
     call, stream = _QUANTIZED_DECODE_CALL.pack(*fields), _stream()
     entry = _fn("mxb_paged_attention_decode_quantized")
     code = entry(call, len(call), stream)

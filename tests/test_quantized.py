@@ -787,3 +787,32 @@ def test_calls_of_nothing(ops):
     ops.read_cache(pool, out, ints([[0, 1]]), ints([0]), ints([0]), ints([-1]))
     assert out.eq(1).all() and torch.equal(pool.scales, before)
     ops.check_status("cuda")
+
+
+@gpu
+@pytest.mark.parametrize("head_dim", [128, 40])
+def test_reaches_beyond_31_bits_limit_nothing(ops, head_dim):
+    """Windows, chunks and kept positions arrive whole: none becomes a small one by losing its upper half."""
+    pool = random_pool(ops, "fp8", 20, 2, 16, head_dim, 3)
+    table, lists = ints([list(range(20))]), (ints([0]), ints([0]), ints([299]))
+    q = torch.randn((1, 4, head_dim), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(BF16)
+    plain, back = torch.zeros_like(q), torch.zeros(pool.shape, dtype=BF16, device="cuda")
+    ops.paged_attention_decode(q, pool, plain, table, *lists, 0.1, 300)
+    ops.read_cache(pool, back, table, ints([0]), ints([299]), ints([299]))
+    for options in (dict(window=2 ** 32 + 5), dict(chunk=2 ** 32 + 7), dict(window=2 ** 31), dict(window=2 ** 31 - 1),
+                    dict(window=3, keep=2 ** 32 + 1), dict(chunk=16, keep=2 ** 31 - 1)):
+        out, read = torch.zeros_like(q), torch.zeros_like(back)
+        ops.paged_attention_decode(q, pool, out, table, *lists, 0.1, 300, **options)
+        ops.read_cache(pool, read, table, ints([0]), ints([299]), ints([299]), **options)
+        assert torch.equal(read, back), options
+        # cuts of the sum differ: two results that are each within a rounding and the halves' 2^-10 of the exact one
+        assert (out.float() - plain.float()).abs().max() <= 2.0 ** -7 * plain.float().abs().max() + 2.0 ** -9 * 4, options
+    ops.check_status("cuda")
+
+
+@gpu
+def test_pools_of_heads_without_values_are_refused(ops):
+    pool = ops.QuantizedPool(torch.zeros((2, 2, 1, 4, 0), dtype=torch.int8, device="cuda"), torch.zeros((2, 2, 1, 4), device="cuda"))
+    k = torch.zeros((1, 0), dtype=BF16, device="cuda")
+    with pytest.raises(ops.KernelError, match="between 1 and 512"):
+        ops.write_cache(k, k, pool, ints([0]), ints([0]))
