@@ -258,3 +258,39 @@ def test_the_command_line(model_folders):
     report = json.loads(run.stdout.strip().splitlines()[-1])
     assert len(report["generated_ids"]) == 8
     assert report["logical_kv_bytes"] == report["cached_tokens"] * 2 * 2 * 2 * (64 + 4)      # layers, planes, heads, a row
+
+
+DESIGNS = [("sadosun", "wide", None), ("sadosun", "bare", None), ("kokolorn", "wide", None), ("kokolorn", "bare", None),
+           ("dimorax", "wide", (0, 1, 3)), ("mekuvik", "wide", (0, 3))]
+
+
+@gpu
+@pytest.mark.parametrize("codes", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("design,name,kept", DESIGNS, ids=lambda v: v if isinstance(v, str) else "")
+def test_other_designs_attend_to_codes_alike_however_cut(design, name, kept, dtype, codes):
+    """Sinks, values turned by position, biases by distance, another layer's keys and values, kept positions, small pages:
+    single tokens read the codes, portions read pages back, and both see the same rows."""
+    import importlib
+    from metallix_b200.config import parse_config
+    from metallix_b200.engine import Engine, StepEntry
+    raw, seed, page, _ = importlib.import_module(f"test_{design}").MODELS[name]
+    if kept is not None:      # without the layers of latent attention, whose rows stay in the compute type
+        raw = {**raw, "layers": [raw["layers"][i] for i in kept]}
+        if raw.get("loop"):
+            raw["loop"] = {**raw["loop"], "start": 0, "stop": len(kept)}
+    requests = {"a": random_ids(3, 75, raw["vocab"]), "b": random_ids(4, 190, raw["vocab"])}
+
+    def logits_of(cache_dtype, steps):
+        engine = Engine.from_random(parse_config(raw), seed, dtype=dtype, page_tokens=page, num_pages=128, max_requests=4,
+                                    cache_dtype=cache_dtype)
+        blank = {k: np.zeros((len(ids), raw["vocab"])) for k, ids in requests.items()}
+        return cuts.replay(engine, steps, blank, StepEntry)[1]
+    plain_rows = logits_of(None, cuts.whole(requests))
+    top = max(np.abs(row).max() for row in plain_rows.values())
+    seen = [logits_of(codes, steps) for steps in (cuts.whole(requests), cuts.tail_by_one(requests, 40), cuts.ragged(requests))]
+    drift = max(float(np.abs(row - seen[0][key]).max()) for other in seen[1:] for key, row in other.items())
+    shift = max(float(np.abs(row - plain_rows[key]).max()) for key, row in seen[0].items())
+    assert shift > 0.0       # the codes were used
+    # float32: as TOL_CODES_F32 says; bfloat16: codes that flip move a logit no further than the codes themselves move it
+    assert drift < (TOL_CODES_F32 * max(top, 1.0) if dtype == "float32" else TOL_BF16_VS_EXACT * max(top, 1.0) + 2 * shift), (drift, shift, top)
