@@ -523,10 +523,10 @@ paged_attention_decode_tma_kernel(const __grid_constant__ CUtensorMap map_cache,
   // the page.
   const int token = row_token[row];
   const int table_row = row_request[row];
+  if (token < 0) return;   // a padding row: its row_request may be anything
   int page = 0;
   if (fetcher && page_key / page_tokens < max_pages)
     page = block_tables[static_cast<size_t>(table_row) * max_pages + page_key / page_tokens];
-  if (token < 0) return;
   const int pos = positions[token];
   const int group = heads / kv_heads;  // <= 8
   const int first_key = first_visible_key(pos, window, chunk);
@@ -735,12 +735,12 @@ paged_attention_decode_resident_kernel(const __grid_constant__ CUtensorMap map_c
   const int which = tid / (pages * HALVES), slot = (tid / HALVES) % pages, half = tid % HALVES;
   const int token = row_token[row];
   const int table_row = row_request[row];
+  if (token < 0) return;   // a padding row: its row_request may be anything
   const int* table = block_tables + static_cast<size_t>(table_row) * max_pages;
   // The page of this block's first tile is asked for together with the
   // position, on the guess that neither a window nor a chunk has moved the first tile.
   int page = 0;
   if (fetcher && rank * pages + slot < max_pages) page = table[rank * pages + slot];
-  if (token < 0) return;   // a padding row
   const int pos = positions[token];
   const int group = heads / kv_heads;  // <= 8
   const int first_key = first_visible_key(pos, window, chunk);

@@ -290,10 +290,10 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
     barrier_init_fence();
   }
   __syncwarp();
+  if (token < 0) return;   // a padding row: its row_request may be anything
   const int* table = a.block_tables + static_cast<size_t>(request) * a.max_pages;
   auto page_at = [&](int key) { return (key >> shift) < a.max_pages ? table[key >> shift] : -1; };
   int box_page = page_at(rank * kSplitKeys + warp * 32 + box_key), scale_page = page_at(rank * kSplitKeys + warp * 32 + scale_key);
-  if (token < 0) return;   // a padding row
   const int pos = a.positions[token];
   const int live = min(group - part * 8, 8), head0 = kv * group + part * 8;   // this block's query heads
   const int first_key = first_visible_key(pos, a.window, a.chunk);

@@ -1899,7 +1899,7 @@ def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
     """Attention of single tokens over their requests' cached keys, split
     along the keys. ``row_token[i]`` is the token (row of q and out) of the
     i-th decoded request, negative for a padding row; ``row_request[i]`` its
-    row of ``block_tables``. ``longest_context`` bounds positions + 1 and
+    row of ``block_tables`` (of a padding row it is not looked at). ``longest_context`` bounds positions + 1 and
     fixes the number of splits. ``partial`` is float32 scratch of
     rows * heads * splits * (head_dim + 2) values, allocated here if absent.
     ``gate`` ([tokens, heads * head_dim] in q's type, rows may be strided):

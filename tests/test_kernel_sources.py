@@ -49,3 +49,27 @@ def test_every_exported_function_is_reached():
     with open(os.path.join(KERNELS, "attention_decode_noalloc.h")) as handle:
         linked = set(re.findall(r"\b(mxb_\w+)\(", handle.read()))
     assert len(exported) > 60 and exported - set(ops._SIGNATURES) - by_hand - linked == set()
+
+
+def decode_kernels():
+    """(name, body) of the decode attention's kernels that look up a row's block table."""
+    out = []
+    for name in ("attention_decode.cu", "attention_decode_quantized.cuh"):
+        with open(os.path.join(KERNELS, name)) as handle:
+            text = re.sub(r"//[^\n]*", "", handle.read())
+        for part in text.split("__global__ void")[1:]:
+            kernel = re.search(r"(\w+)\s*\(\s*const", part)
+            body = part.split("\n}\n")[0]
+            if "row_request[row]" in body:
+                out.append((kernel.group(1), body))
+    return out
+
+
+def test_a_padding_rows_table_is_not_looked_up():
+    """A row without a token has no row of the block tables either: ``row_request`` of one may lie outside them."""
+    kernels = decode_kernels()
+    assert len(kernels) >= 5
+    for name, body in kernels:
+        left = body.index("if (token < 0)")
+        reads = [m.start() for m in re.finditer(r"\btable\[|\bblock_tables\[|\bpage_at\(|\bquantized_row\(", body)]
+        assert reads and left < min(reads), name

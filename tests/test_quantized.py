@@ -816,3 +816,31 @@ def test_pools_of_heads_without_values_are_refused(ops):
     k = torch.zeros((1, 0), dtype=BF16, device="cuda")
     with pytest.raises(ops.KernelError, match="between 1 and 512"):
         ops.write_cache(k, k, pool, ints([0]), ints([0]))
+
+
+@gpu
+@pytest.mark.parametrize("head_dim,heads,kv_heads,page", [(128, 8, 2, 16), (64, 7, 1, 8), (256, 4, 2, 32), (40, 4, 2, 4), (128, 4, 2, 3)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["fp8", None])
+@pytest.mark.parametrize("longest", [70, 5000])
+def test_a_padding_rows_request_is_not_looked_at(ops, kind, dtype, head_dim, heads, kv_heads, page, longest):
+    """Padding rows whose request lies outside the block tables, over codes and over a cache in the compute type: bit for
+    bit what padding rows of request 0 give."""
+    if kind is None and not ops.decode_attention_supported(head_dim, heads, kv_heads, dtype):
+        pytest.skip("the split-key kernel does not take this layout")
+    lengths = [longest, 3]
+    pages, table = spread_tables(lengths, page, 1)
+    pool = random_pool(ops, "fp8", pages, kv_heads, page, head_dim, 2)
+    if kind is None:
+        pool = values_of(pool).to(dtype)
+    q = torch.randn((4, heads, head_dim), generator=torch.Generator(device="cuda").manual_seed(9), device="cuda").to(dtype)
+    positions = ints([2, 0, longest - 1, 0])
+    outs = []
+    for filler in ([0, 0, 0], [-1, 2 ** 30, -2 ** 31], [2 ** 31 - 1, 2, -5]):
+        out = torch.full(q.shape, 5.0, dtype=dtype, device="cuda")
+        ops.paged_attention_decode(q, pool, out, table, ints([-1, 2, -7, 0, -2 ** 31]), ints([filler[0], 0, filler[1], 1, filler[2]]),
+                                   positions, 0.1, longest)
+        outs.append(out)
+    ops.check_status("cuda")
+    assert outs[0][[1, 3]].eq(5.0).all() and not outs[0][[0, 2]].eq(5.0).all()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
