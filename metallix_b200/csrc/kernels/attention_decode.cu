@@ -1322,8 +1322,11 @@ struct QuantizedDecodeCall {
 // page_tokens, head_dim] and scales [pages, 2, kv_heads, page_tokens]. With w
 // (bfloat16 heads of 64 or 128 values, up to 64 tokens) the partial results are
 // put together and projected by one kernel, as mxb_paged_attention_decode_project does.
-// settled: with chained launches on, the positions ahead of each token's own were
-// written by launches before the last one, and may be fetched while that one runs.
+// settled: the positions ahead of each token's own were complete when the launch
+// right ahead of this one began, and with chained launches on may be fetched while
+// that one runs. Chained launches start before the ones ahead of them have ended, so
+// rows that an earlier one of them wrote are complete only behind a copy, a
+// synchronisation or a launch of another kind.
 // partial (float32, rows * heads * max_splits * (head_dim + 2) values) may be null:
 // where it is needed, cudaErrorNotReady says so and nothing has been launched.
 MXB_API int mxb_paged_attention_decode_quantized(const void* call, int bytes, cudaStream_t stream) {

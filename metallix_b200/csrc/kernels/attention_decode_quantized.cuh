@@ -28,7 +28,7 @@ struct QuantizedDecode {
   ScoreBias bias;
   int group;                     // query heads a key/value head
   int page_shift;                // log2 of page_tokens, -1 where that is no power of two
-  int settled;                   // the positions ahead of each token's own were written by launches before the last one
+  int settled;                   // the positions ahead of each token's own were complete when the launch ahead of this one began
   int* status;
   // What the blocks of a cluster write where they put their results together themselves (`fused`: the slots of a pair are one cluster).
   int fused, max_splits;
@@ -379,7 +379,7 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
     asm volatile("cp.async.commit_group;\n" ::);
   };
   // The token's own row, of the walk's last tile, is written by the kernel ahead of this one; with `settled` all others
-  // are older, and their copies start ahead of the wait.
+  // were complete when that kernel began, and their copies start ahead of the wait.
   bool waited = !a.settled;
   if (walk.tile(rank) != rank) {
     box_page = page_of(0, box_key);

@@ -334,7 +334,7 @@ constexpr int kReadBlocks = 8 * 148 * 8;   // of a launch, at most (or one a req
 template <typename T, int KIND>
 __global__ void __launch_bounds__(kReadThreads)
 read_cache_pieces_kernel(const __grid_constant__ ReadArgs a) {
-  // No release ahead of the end: what follows may read `out` as a cache whose pages it takes to be settled.
+  // No release ahead of the end: what follows has nothing to do before `out` is there.
   chain_wait();   // the codes are the work of kernels ahead
   const int row = blockIdx.y, end = a.last[row], head_dim = a.head_dim, page_tokens = a.page_tokens;
   if (end < 0) return;

@@ -1396,7 +1396,8 @@ def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tenso
     attention kernels take them), up to position ``last[i]``. ``out`` (float32
     or bfloat16) has the pool's shape: a page keeps its number, so the same
     block tables serve it; rows that are not read stay as they are. A negative
-    ``last`` reads nothing."""
+    ``last`` reads nothing. The prompt kernels may follow at once; for
+    ``paged_attention_decode`` over ``out`` see its ``settled``."""
     _need(isinstance(pool, QuantizedPool), "pool must be a QuantizedPool")
     codes, shape, device = pool.codes, pool.shape, pool.device_index
     rows = row_request.numel() if isinstance(row_request, torch.Tensor) else 0
@@ -1911,9 +1912,13 @@ def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
     first that many positions are seen beside the window or chunk. ``cache`` may
     be a ``QuantizedPool``, with heads of any size up to 256 and any number of
     query heads a key/value head; then ``settled`` says that the positions ahead
-    of each token's own were written by launches before the last one, so that
-    with chained launches on they may be fetched while that one runs (a cache in
-    the compute type is taken to be so)."""
+    of each token's own were complete, whatever wrote them finished, when the
+    launch right ahead of this one began, so that with chained launches on they
+    may be fetched while that one runs. That an earlier launch wrote them is not
+    enough, because chained launches overlap one another: between the last such
+    write and the launch right ahead there has to be a copy, a synchronisation or
+    a launch that is not chained (an engine's steps begin with a copy). A cache in
+    the compute type is always taken to be so."""
     if isinstance(cache, QuantizedPool):
         _need(out is not None, "out must be a tensor")
         _decode_quantized(q, cache, out, block_tables, row_token, row_request, positions, scale, longest_context, window,

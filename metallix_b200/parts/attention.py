@@ -198,7 +198,9 @@ def attend_cached(q_heads: torch.Tensor, cache: CacheView, ctx: StepContext, *, 
     values of a head's keys and values are in use (0: all), the others being zeros.
     Of a cache held as codes, single tokens read the codes, which takes
     ``split_decode``; for portions of prompts the pages that they see are read back
-    into the compute type first."""
+    into the compute type first. ``settled``: positions ahead of a single token's own
+    were written in earlier steps, and a step's integers are copied to the device
+    ahead of its launches, which waits for all of the step before."""
     tokens, heads, head_dim = q_heads.shape
     coded = isinstance(cache.pool, ops.QuantizedPool)
     if flash and head_dim == 256:

@@ -844,3 +844,53 @@ def test_a_padding_rows_request_is_not_looked_at(ops, kind, dtype, head_dim, hea
     ops.check_status("cuda")
     assert outs[0][[1, 3]].eq(5.0).all() and not outs[0][[0, 2]].eq(5.0).all()
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def close_as_halves(out, exact, bound, dtype, keys):
+    """What the tensor-core form owes: bfloat16 queries' weights are halves (2^-11 each; below 2^-14, with the largest at
+    2^6 or above, 2^-31 of the largest), float32 queries' two halves (2^-22); the rest as in ``close``."""
+    per_weight = (2.0 ** -11 if dtype == BF16 else 2.0 ** -22) + 30 * 8 * 2.0 ** -24
+    least = keys * 2.0 ** -31 * bound.amax(-1, keepdim=True)
+    off = (out.double() - exact).abs()
+    limit = per_weight * bound + least + HALF[dtype] * exact.abs() * 1.01 + 1e-30
+    assert (off <= limit).all(), f"{(off / limit).max().item():.2f} times the bound"
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim,heads,kv_heads,page", [(64, 7, 1, 8), (128, 8, 2, 16), (256, 4, 2, 32)])
+@pytest.mark.parametrize("options", [dict(), dict(window=900), dict(window=200, keep=300), dict(chunk=512)],
+                         ids=lambda o: "-".join(f"{k}{v}" for k, v in o.items()) or "all")
+def test_settled_positions_and_a_row_written_right_ahead(ops, kind, dtype, head_dim, heads, kv_heads, page, options):
+    """A step as an engine makes it, with overlapping launches on: contexts written earlier, a copy, the tokens' own rows,
+    and the attention, told that the contexts are settled. Against the definition, not against another run."""
+    lengths = [1500, 1, 129, 700, 2048, 33]
+    rows = len(lengths)
+    pages, table = spread_tables(lengths, page, 2)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    at = torch.cat([torch.arange(n) for n in lengths])
+    request = torch.cat([torch.full((n,), r) for r, n in enumerate(lengths)])
+    slots = table.cpu().long()[request, at // page] * page + at % page
+    own = at == torch.tensor(lengths)[request] - 1
+    q = torch.randn((rows, heads, head_dim), generator=gen, device="cuda").to(dtype)
+    positions, lists = ints([n - 1 for n in lengths]), ints(range(rows))
+    host, older, newer = positions.cpu().pin_memory(), (~own).cuda(), own.cuda()
+    slots_of = [slots[m].to(torch.int32).cuda() for m in (~own, own)]
+    try:
+        ops.set_chained_launches(True)
+        for turn in range(3):
+            pool = random_pool(ops, kind, pages, kv_heads, page, head_dim, 50 + turn)      # earlier owners' rows
+            k, v = (torch.randn((len(at), kv_heads * head_dim), generator=gen, device="cuda").to(dtype) for _ in range(2))
+            out = torch.zeros_like(q)
+            parts = [(k[m], v[m]) for m in (older, newer)]
+            wheres = [at[m].to(torch.int32).cuda() for m in (~own, own)]
+            torch.cuda.synchronize()
+            ops.write_cache(*parts[0], pool, slots_of[0], wheres[0])
+            positions.copy_(host, non_blocking=True)       # a step's integers
+            ops.write_cache(*parts[1], pool, slots_of[1], wheres[1])
+            ops.paged_attention_decode(q, pool, out, table, lists, lists, positions, 0.1, max(lengths), settled=True, **options)
+            ops.check_status("cuda")
+            close_as_halves(out, *exact_decode(q, pool, table, [(r, r) for r in range(rows)], positions, 0.1, **options), dtype, max(lengths))
+    finally:
+        ops.set_chained_launches(False)
