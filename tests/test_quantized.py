@@ -894,3 +894,20 @@ def test_settled_positions_and_a_row_written_right_ahead(ops, kind, dtype, head_
             close_as_halves(out, *exact_decode(q, pool, table, [(r, r) for r in range(rows)], positions, 0.1, **options), dtype, max(lengths))
     finally:
         ops.set_chained_launches(False)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("head_dim,heads,kv_heads,page", [(64, 14, 2, 32), (128, 16, 2, 16), (256, 5, 1, 8)])
+@pytest.mark.parametrize("longest", [40, 900, 6000])
+def test_weights_are_halves(ops, kind, head_dim, heads, kv_heads, page, longest):
+    """bfloat16 outputs to within the eleven bits that weights are held in."""
+    lengths = [longest, longest // 3 + 1, 1]
+    pages, table = spread_tables(lengths, page, 4)
+    pool = random_pool(ops, kind, pages, kv_heads, page, head_dim, 8)
+    q = (1.5 * torch.randn((3, heads, head_dim), generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")).to(BF16)
+    positions, lists, out = ints([n - 1 for n in lengths]), ints(range(3)), torch.zeros_like(q)
+    scale = 1.0 / math.sqrt(head_dim)
+    ops.paged_attention_decode(q, pool, out, table, lists, lists, positions, scale, longest)
+    ops.check_status("cuda")
+    close_as_halves(out, *exact_decode(q, pool, table, [(r, r) for r in range(3)], positions, scale), BF16, longest)
