@@ -287,7 +287,10 @@ paged_attention_decode_mma_kernel(const __nv_bfloat16* __restrict__ q, const __n
   // runs, copies included, while the kernels before this one are still at work.
   const int split = blockIdx.x, kv = blockIdx.y, row = blockIdx.z;
   const int token = row_token[row];
-  if (token < 0) return;
+  if (token < 0) {
+    chain_wait();   // a launch that ends ahead of the one before it lets what follows start too early
+    return;
+  }
   const int pos = positions[token];
   const int group = heads / kv_heads;  // <= 8
   const int first_key = first_visible_key(pos, window, chunk);
@@ -523,7 +526,10 @@ paged_attention_decode_tma_kernel(const __grid_constant__ CUtensorMap map_cache,
   // the page.
   const int token = row_token[row];
   const int table_row = row_request[row];
-  if (token < 0) return;   // a padding row: its row_request may be anything
+  if (token < 0) {   // a padding row: its row_request may be anything
+    chain_wait();
+    return;
+  }
   int page = 0;
   if (fetcher && page_key / page_tokens < max_pages)
     page = block_tables[static_cast<size_t>(table_row) * max_pages + page_key / page_tokens];
@@ -735,7 +741,10 @@ paged_attention_decode_resident_kernel(const __grid_constant__ CUtensorMap map_c
   const int which = tid / (pages * HALVES), slot = (tid / HALVES) % pages, half = tid % HALVES;
   const int token = row_token[row];
   const int table_row = row_request[row];
-  if (token < 0) return;   // a padding row: its row_request may be anything
+  if (token < 0) {   // a padding row: its row_request may be anything
+    chain_wait();
+    return;
+  }
   const int* table = block_tables + static_cast<size_t>(table_row) * max_pages;
   // The page of this block's first tile is asked for together with the
   // position, on the guess that neither a window nor a chunk has moved the first tile.
@@ -966,7 +975,11 @@ paged_attention_merge_kernel(const float* __restrict__ partial, T* __restrict__ 
   chain_release();
   const int row = blockIdx.x, head = blockIdx.y, d = threadIdx.x;
   const int token = row_token[row];  // the step's integers are not written by any kernel of the step
-  if (token < 0 || d >= head_dim) return;
+  if (d >= head_dim) return;
+  if (token < 0) {
+    chain_wait();
+    return;
+  }
   const int pos = positions[token];
   const int first_key = first_visible_key(pos, window, chunk);
   const KeyWalk walk = key_walk(first_key, pos, keep, kSplitKeys);
@@ -974,6 +987,7 @@ paged_attention_merge_kernel(const float* __restrict__ partial, T* __restrict__ 
     // The caller's bound on the contexts does not cover this row: its partial
     // results lie outside what the scratch was sized for. The row is left as it is.
     if (d == 0) atomicOr(status, kStatusBadSlot);
+    chain_wait();
     return;
   }
   // One partial result per split of 128 keys, or (slots > 0) per block of the

@@ -290,7 +290,10 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
     barrier_init_fence();
   }
   __syncwarp();
-  if (token < 0) return;   // a padding row: its row_request may be anything
+  if (token < 0) {   // a padding row: its row_request may be anything
+    chain_wait();    // a launch that ends ahead of the one before it lets what follows start too early
+    return;
+  }
   const int* table = a.block_tables + static_cast<size_t>(request) * a.max_pages;
   auto page_at = [&](int key) { return (key >> shift) < a.max_pages ? table[key >> shift] : -1; };
   int box_page = page_at(rank * kSplitKeys + warp * 32 + box_key), scale_page = page_at(rank * kSplitKeys + warp * 32 + scale_key);
@@ -300,6 +303,7 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
   const KeyWalk walk = key_walk(first_key, pos, a.keep, kSplitKeys);
   if (pos / kSplitKeys >= a.max_splits) {   // beyond the caller's bound on the contexts: the row is left as it is
     if (a.fused && rank == 0 && threadIdx.x == 0) atomicOr(a.status, kStatusBadSlot);
+    chain_wait();
     return;
   }
   // The end of a pair whose blocks are a cluster: every block's partial result lies at `results` in its shared memory,

@@ -73,3 +73,21 @@ def test_a_padding_rows_table_is_not_looked_up():
         left = body.index("if (token < 0)")
         reads = [m.start() for m in re.finditer(r"\btable\[|\bblock_tables\[|\bpage_at\(|\bquantized_row\(", body)]
         assert reads and left < min(reads), name
+
+
+def test_rows_of_padding_keep_the_chain():
+    """A kernel that may start ahead of the end of the one before it waits for that in every row. One that left without
+    (with padding alone) would end first, and what waits for it would not find the work of the kernel before."""
+    names = []
+    for name in ("attention_decode.cu", "attention_decode_quantized.cuh"):
+        with open(os.path.join(KERNELS, name)) as handle:
+            text = re.sub(r"//[^\n]*", "", handle.read())
+        for part in text.split("__global__ void")[1:]:
+            body = part.split("\n}\n")[0]
+            if "chain_wait()" not in body:
+                continue      # launched the ordinary way: nothing starts ahead of its end
+            names.append(re.search(r"(\w+)\s*\(\s*const", part).group(1))
+            assert re.search(r"if \(token < 0\) \{\s*chain_wait\(\);\s*return;", body), names[-1]
+            for bound in re.finditer(r"kSplitKeys >= (a\.)?max_splits\) \{(.*?)return;", body, re.S):
+                assert "chain_wait();" in bound.group(2), names[-1]
+    assert len(names) >= 5

@@ -911,3 +911,34 @@ def test_weights_are_halves(ops, kind, head_dim, heads, kv_heads, page, longest)
     ops.paged_attention_decode(q, pool, out, table, lists, lists, positions, scale, longest)
     ops.check_status("cuda")
     close_as_halves(out, *exact_decode(q, pool, table, [(r, r) for r in range(3)], positions, scale), BF16, longest)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("padding,longest", [(1, 100), (3, 9000), (40, 9000)])
+def test_attention_of_padding_alone_keeps_the_order_of_launches(ops, kind, padding, longest):
+    """Overlapping launches: a write of whole contexts, an attention whose rows are all padding, and pages read back, which
+    wait for the write although the attention between had nothing to do."""
+    page, length, rows, kv_heads, head_dim = 16, 2000, 6, 4, 128
+    pages, table = spread_tables([length] * rows, page, 2)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    at = torch.arange(length).repeat(rows)
+    slots = (table.cpu().long()[torch.arange(rows).repeat_interleave(length), at // page] * page + at % page).to(torch.int32).cuda()
+    at = at.to(torch.int32).cuda()
+    q, out = (torch.zeros((padding, 8, head_dim), dtype=BF16, device="cuda") for _ in range(2))
+    none, lists, last = ints([-1] * padding), ints(range(rows)), ints([length - 1] * rows)
+    zeros, first = ints([0] * padding), ints([0] * rows)
+    try:
+        ops.set_chained_launches(True)
+        for turn in range(6):
+            pool = ops.QuantizedPool.zeros(pages, kv_heads, page, head_dim, codes=kind)
+            k, v = (torch.randn((rows * length, kv_heads * head_dim), generator=gen, device="cuda").to(BF16) for _ in range(2))
+            back = torch.zeros(pool.shape, dtype=F32, device="cuda")
+            torch.cuda.synchronize()
+            ops.write_cache(k, v, pool, slots, at)
+            ops.paged_attention_decode(q, pool, out, table, none, zeros, zeros, 0.1, longest, settled=True)
+            ops.read_cache(pool, back, table, lists, first, last)
+            ops.check_status("cuda")
+            assert torch.equal(back, values_of(pool).float()) and out.eq(0).all()
+    finally:
+        ops.set_chained_launches(False)
