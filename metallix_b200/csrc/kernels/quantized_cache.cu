@@ -342,14 +342,16 @@ read_cache_pieces_kernel(const __grid_constant__ ReadArgs a) {
   const int per_row = head_dim >> 4, rows = 2 * a.kv_heads * page_tokens, pieces = rows * per_row;
   const int per_page = (pieces + kReadPieces - 1) / kReadPieces;
   const int* table = a.block_tables + static_cast<size_t>(a.row_request[row]) * a.max_pages;
-  for (int item = blockIdx.x; item < walk.count * per_page; item += gridDim.x) {
+  const int steps = min(walk.count, a.max_pages + 1);   // as many as the table has pages, and one that finds that there are no more
+  for (int item = blockIdx.x; item < steps * per_page; item += gridDim.x) {
     const int step = item / per_page, slot = walk.tile(step), piece0 = (item - step * per_page) * kReadPieces;
     const int page = slot < a.max_pages ? table[slot] : -1;
     if (page < 0 || page >= a.num_pages) {
       if (threadIdx.x == 0) atomicOr(a.status, kStatusBadPage);
+      if (slot >= a.max_pages) break;   // `last` lies beyond the table, and so do all further steps
       continue;
     }
-    const int seen = end - slot * page_tokens + 1;   // rows of the page up to the last position
+    const int seen = min(end - slot * page_tokens, page_tokens - 1) + 1;   // rows of the page up to the last position
     const size_t base = static_cast<size_t>(page) * rows;
     const uint4* src = reinterpret_cast<const uint4*>(a.codes + base * head_dim);
     uint4 held[kReadDepth];
@@ -384,14 +386,18 @@ read_cache_kernel(const __grid_constant__ ReadArgs a) {
   chain_wait();
   const int slot = blockIdx.x, row = blockIdx.y;
   const int begin = first_visible_key(max(a.first[row], 0), a.window, a.chunk), end = a.last[row];
+  if (end < 0) return;
+  const int last_slot = end / a.page_tokens;
+  if (slot == 0 && last_slot >= a.max_pages && threadIdx.x == 0) atomicOr(a.status, kStatusBadPage);   // `last` lies beyond the table
+  if (slot > last_slot || slot >= a.max_pages) return;
   const int key0 = slot * a.page_tokens;
-  if (key0 > end || (key0 + a.page_tokens <= begin && key0 >= a.keep)) return;
+  if (key0 + a.page_tokens <= begin && key0 >= a.keep) return;
   const int page = a.block_tables[static_cast<size_t>(a.row_request[row]) * a.max_pages + slot];
   if (page < 0 || page >= a.num_pages) {
     if (threadIdx.x == 0) atomicOr(a.status, kStatusBadPage);
     return;
   }
-  const int rows = min(a.page_tokens, end - key0 + 1);
+  const int rows = min(end - key0, a.page_tokens - 1) + 1;
   const size_t base = static_cast<size_t>(page) * 2 * a.kv_heads * a.page_tokens;
   for (int i = threadIdx.x; i < 2 * a.kv_heads * rows * a.head_dim; i += blockDim.x) {
     const int line = i / a.head_dim, d = i - line * a.head_dim;
@@ -500,14 +506,15 @@ struct ReadCall {
 // query at position first[i] or later sees (window, chunk, keep as in the
 // attention kernels), up to position last[i], from the pool into `out`, which
 // has the pool's layout [pages, 2, kv_heads, page_tokens, head_dim] in `dtype`.
+// Positions beyond the table are reported (a bad page); what the table has of them is read.
 MXB_API int mxb_read_cache(const void* call, int bytes, cudaStream_t stream) {
   if (bytes != static_cast<int>(sizeof(ReadCall))) return static_cast<int>(cudaErrorInvalidValue);
   const ReadCall& c = *static_cast<const ReadCall*>(call);
-  if (c.rows <= 0 || c.max_pages <= 0) return 0;
+  if (c.rows <= 0) return 0;
   const int kind = static_cast<int>(c.kind), dtype = static_cast<int>(c.dtype), rows = static_cast<int>(c.rows),
             kv_heads = static_cast<int>(c.kv_heads), head_dim = static_cast<int>(c.head_dim), max_pages = static_cast<int>(c.max_pages),
             page_tokens = static_cast<int>(c.page_tokens), num_pages = static_cast<int>(c.num_pages);
-  if (rows > 65535 || !pool_fits(num_pages, kv_heads, page_tokens) || head_dim <= 0 || head_dim > 512 ||
+  if (rows > 65535 || max_pages < 0 || !pool_fits(num_pages, kv_heads, page_tokens) || head_dim <= 0 || head_dim > 512 ||
       2LL * kv_heads * page_tokens * head_dim > 0x7fffffffLL ||   // a page's codes are counted in 31 bits
       (dtype != kF32 && dtype != kBF16) || (kind != kCodesE4M3 && kind != kCodesInt8))
     return static_cast<int>(cudaErrorInvalidValue);
@@ -515,7 +522,8 @@ MXB_API int mxb_read_cache(const void* call, int bytes, cudaStream_t stream) {
   // A block an item where tables are short; wide tables of short contexts (a captured step's) walk with a stride instead.
   const long long items = static_cast<long long>(max_pages) * ((2LL * kv_heads * page_tokens * (head_dim / 16) + kReadPieces - 1) / kReadPieces);
   const long long most = kReadBlocks / rows > 0 ? kReadBlocks / rows : 1;
-  const dim3 grid(static_cast<unsigned>(!by_pieces ? max_pages : (items < most ? items : most)), rows);
+  const long long blocks = !by_pieces ? max_pages : (items < most ? items : most);
+  const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1), rows);   // a table without pages: a block that says so
   const ReadArgs args = {static_cast<const uint8_t*>(c.codes), c.scales, c.out, c.block_tables, max_pages, c.row_request, c.first, c.last,
                          kv_heads, head_dim, page_tokens, num_pages, static_cast<int>(c.window), static_cast<int>(c.chunk),
                          static_cast<int>(c.keep), c.status};

@@ -1396,7 +1396,7 @@ def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tenso
     attention kernels take them), up to position ``last[i]``. ``out`` (float32
     or bfloat16) has the pool's shape: a page keeps its number, so the same
     block tables serve it; rows that are not read stay as they are. A negative
-    ``last`` reads nothing. The prompt kernels may follow at once; for
+    ``last`` reads nothing; one beyond the table is reported, like a page outside the pool. The prompt kernels may follow at once; for
     ``paged_attention_decode`` over ``out`` see its ``settled``."""
     _need(isinstance(pool, QuantizedPool), "pool must be a QuantizedPool")
     codes, shape, device = pool.codes, pool.shape, pool.device_index

@@ -942,3 +942,32 @@ def test_attention_of_padding_alone_keeps_the_order_of_launches(ops, kind, paddi
             assert torch.equal(back, values_of(pool).float()) and out.eq(0).all()
     finally:
         ops.set_chained_launches(False)
+
+
+@gpu
+@pytest.mark.parametrize("head_dim,offset", [(64, 0), (40, 0), (64, 1)])
+@pytest.mark.parametrize("last", [8, 11, 4000, 2 ** 31 - 1])
+@pytest.mark.parametrize("options", [dict(), dict(window=3), dict(keep=2, window=1)], ids=lambda o: "-".join(f"{k}{v}" for k, v in o.items()) or "all")
+def test_positions_beyond_the_table_are_reported(ops, head_dim, offset, last, options):
+    """By either kernel that reads pages back; what the table has of them is read, nothing else is written."""
+    made = random_pool(ops, "fp8", 5, 2, 4, head_dim, 1)
+    room = torch.zeros(made.codes.numel() + 16, dtype=torch.uint8, device="cuda")
+    codes = room[offset:offset + made.codes.numel()].view(torch.float8_e4m3fn).view(made.shape)
+    codes.view(torch.uint8).copy_(made.codes.view(torch.uint8))
+    pool, table = ops.QuantizedPool(codes, made.scales), ints([[1, 3]])
+    zero, far = ints([0]), ints([last])
+    expect = torch.full(pool.shape, 7.0, device="cuda")
+    expect[[1, 3]] = values_of(pool)[[1, 3]].float()
+    out = torch.full(pool.shape, 7.0, device="cuda")
+    ops.read_cache(pool, out, table, zero, zero, far, **options)
+    with pytest.raises(ops.KernelError, match="block-table"):
+        ops.check_status("cuda")
+    assert torch.equal(out, expect)
+    for tables, end in ((table, 7), (torch.empty((1, 0), dtype=torch.int32, device="cuda"), -1)):
+        ops.read_cache(pool, out, tables, zero, zero, ints([end]), **options)
+        ops.check_status("cuda")
+    assert torch.equal(out, expect)
+    ops.read_cache(pool, out, torch.empty((1, 0), dtype=torch.int32, device="cuda"), zero, zero, zero, **options)
+    with pytest.raises(ops.KernelError, match="block-table"):
+        ops.check_status("cuda")
+    assert torch.equal(out, expect)
