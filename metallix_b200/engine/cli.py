@@ -77,7 +77,8 @@ def build_parser() -> argparse.ArgumentParser:
     gen.add_argument("--eos-ids", type=_ids, help="stop ids; default: the configuration's")
     gen.add_argument("--ignore-eos", action="store_true")
     gen.add_argument("--verify-cache", action="store_true",
-                     help="recompute every generated position from the whole sequence and compare")
+                     help="recompute every generated position from the whole sequence and compare "
+                          "(with 8-bit codes also without them)")
     gen.add_argument("--gemm", choices=("auto", "tcgen05", "cublas", "simple"), default="auto")
     gen.add_argument("--trace-out", metavar="FILE",
                      help="write a Chrome/Perfetto JSON timeline of the steps (host and device spans)")
@@ -92,9 +93,23 @@ def build_parser() -> argparse.ArgumentParser:
 
 
 VERIFY_BOUNDS = {"float32": (5e-4, 1e-4), "bfloat16": (0.0, 2.5e-2)}   # (absolute, relative to the row's largest |logit|)
+# Over a cache of 8-bit codes two right engines differ by more: a quotient near the middle between two codes gets the one
+# here and the other there, each as near to the number itself. So either engine is off the logits without codes by about
+# as much as the codes move a logit, and the two from one another by no more than twice that.
+CODES_SHIFTS = 2.0
 
 
-def _verify_cache(engine, checker, result, dtype: str) -> dict:
+def _whole_logits(engine, result):
+    """Logits of every generated position, from the whole sequence in one step."""
+    from .engine import StepEntry
+    ids = list(result.input_ids) + list(result.generated_ids[:-1])
+    logits = engine.step([StepEntry("verify-cache", ids, list(range(len(result.input_ids) - 1, len(ids))))]).clone()
+    engine.check()
+    engine.release("verify-cache")
+    return logits
+
+
+def _verify_cache(engine, checker, result, dtype: str, uncoded=None) -> dict:
     """Recomputes the logits of every generated position twice over and
     compares them, as the reference's ``--verify-cache`` compares cached and
     uncached logits (crates/app/cli/src/qwen_forward.rs:916-939): once with
@@ -102,29 +117,31 @@ def _verify_cache(engine, checker, result, dtype: str) -> dict:
     cache), and once with ``checker``, a second engine over the same weights
     that runs other kernels end to end (no captured graphs, no overlapped
     launches, matrix products on CUDA cores instead of tensor cores or the
-    library), so that an error the serving paths share does not hide."""
-    import torch
+    library), so that an error the serving paths share does not hide. Over a
+    cache of 8-bit codes ``uncoded`` holds the logits of an engine like
+    ``checker`` without codes: what the codes move a logit by joins the bound,
+    and is reported, since the two engines' difference does not show it."""
     from .. import ops
-    from .engine import StepEntry
-    ids = list(result.input_ids) + list(result.generated_ids[:-1])
-    first = len(result.input_ids) - 1
-    wanted = list(range(first, len(ids)))
-    whole = engine.step([StepEntry("verify-cache", ids, wanted)]).clone()
+    whole = _whole_logits(engine, result)
     picked = ops.argmax(whole).tolist()
-    engine.check()
-    engine.release("verify-cache")
-    other = checker.step([StepEntry("verify-cache", ids, wanted)])
-    checker.check()
-    checker.release("verify-cache")
+    other = _whole_logits(checker, result)
     absolute, relative = VERIFY_BOUNDS[dtype]
     difference = (whole.double() - other.double()).abs()
     magnitude = other.double().abs().amax(dim=1, keepdim=True)
     bound = absolute + relative * (other.double().abs() if dtype == "float32" else magnitude)
+    bounds, codes = {"absolute": absolute, "relative": relative}, {}
+    if uncoded is not None:
+        shift = (other.double() - uncoded.to(other.device).double()).abs()
+        bound = bound + CODES_SHIFTS * shift.max()
+        bounds["of_codes_shift"] = CODES_SHIFTS
+        codes = {"max_abs_logit_shift_of_codes": float(shift.max()),
+                 "max_shift_of_codes_of_row_magnitude": float((shift / magnitude).max())}
     return {"positions": len(picked), "greedy_tokens_match": picked == list(result.generated_ids),
             "max_abs_logit_difference": float(difference.max()),
             "max_difference_of_row_magnitude": float((difference / magnitude).max()),
+            **codes,
             "logits_within_bound": bool((difference <= bound).all()),
-            "bound": {"absolute": absolute, "relative": relative},
+            "bound": bounds,
             "checked_against": "a second engine: eager launches, CUDA-core matrix products"}
 
 
@@ -179,15 +196,23 @@ def run_gen(args) -> int:
                        deadline_s=args.generation_timeout_ms / 1e3 if args.generation_timeout_ms > 0 else None)
     from ..config.registry import resolve
     family = resolve(config.to_dict()).model_type   # "qwen3": the reference's receipts name the family so
-    checker, verified = None, True
+    checker, verified, uncoded = None, True, {}
     if args.verify_cache and not args.sample:
         checker_options = dict(options, cuda_graphs=False, chained_launches=False, gemm_backend="simple")
         longest = max(len(r.input_ids) + len(r.generated_ids) for r in results)
         checker_options["num_pages"] = -(-longest // args.block_size) + 1
         checker_options.pop("pool_bytes", None)
-        checker = (Engine.from_folder(args.model, **checker_options) if args.model
-                   else Engine.from_random(config, args.random_weights, **checker_options))
-    for result in results:
+
+        def second_engine(**options):
+            options = dict(checker_options, **options)
+            return (Engine.from_folder(args.model, **options) if args.model
+                    else Engine.from_random(config, args.random_weights, **options))
+        if args.cache_dtype != "auto":
+            bare = second_engine(cache_dtype="auto")
+            uncoded = {i: _whole_logits(bare, result).cpu() for i, result in enumerate(results) if not result.failed}
+            del bare   # its weights make room for the checker's
+        checker = second_engine()
+    for index, result in enumerate(results):
         report = {
             "schema_version": 1,
             "operation": f"{family}_sampled_cached_generation" if args.sample
@@ -208,7 +233,7 @@ def run_gen(args) -> int:
                                   "seed": args.seed, "temperature": args.temperature,
                                   "top_p": args.top_p, "top_k": args.top_k}
         if args.verify_cache and not args.sample and not result.failed:
-            report["cache_comparisons"] = _verify_cache(engine, checker, result, args.dtype)
+            report["cache_comparisons"] = _verify_cache(engine, checker, result, args.dtype, uncoded.get(index))
             verified = verified and report["cache_comparisons"]["logits_within_bound"]
         print(json.dumps(report), flush=True)
         if args.verbose:

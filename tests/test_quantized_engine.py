@@ -294,3 +294,51 @@ def test_other_designs_attend_to_codes_alike_however_cut(design, name, kept, dty
     assert shift > 0.0       # the codes were used
     # float32: as TOL_CODES_F32 says; bfloat16: codes that flip move a logit no further than the codes themselves move it
     assert drift < (TOL_CODES_F32 * max(top, 1.0) if dtype == "float32" else TOL_BF16_VS_EXACT * max(top, 1.0) + 2 * shift), (drift, shift, top)
+
+
+# Matrices large enough for the float32 products on the tensor cores, so that a second engine's are not the same to the bit.
+CHECKED = dict(architectures=["Qwen3ForCausalLM"], model_type="qwen3", hidden_act="silu", num_hidden_layers=4, hidden_size=1024,
+               num_attention_heads=16, num_key_value_heads=8, head_dim=128, intermediate_size=2048, vocab_size=2000,
+               rope_theta=10000.0, rms_norm_eps=1e-6, tie_word_embeddings=True, max_position_embeddings=4096)
+
+
+@gpu
+@pytest.mark.parametrize("codes", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_command_line_checks_a_cache_of_codes(tmp_path, dtype, codes):
+    """Two engines whose products differ in the last bits code a number here and there otherwise: that is no fault, and
+    what the codes themselves move is in the report."""
+    path = tmp_path / "config.json"
+    path.write_text(json.dumps(CHECKED))
+    command = [sys.executable, os.path.join(ROOT, "bin", "mxb"), "gen", "--config", str(path), "--random-weights", "3", "--input-ids",
+               ",".join(map(str, random_ids(9, 60, CHECKED["vocab_size"]))), "--max-tokens", "24", "--dtype", dtype, "--ignore-eos",
+               "--num-pages", "64", "--cache-dtype", codes, "--verify-cache"]
+    run = subprocess.run(command, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=600, cwd=ROOT)
+    assert run.returncode == 0, (run.stdout[-2000:], run.stderr[-2000:])
+    report = json.loads(run.stdout.strip().splitlines()[-1])["cache_comparisons"]
+    assert report["logits_within_bound"] is True and report["positions"] == 24
+    assert 0.0 < report["max_abs_logit_shift_of_codes"] and report["max_abs_logit_difference"] <= 2 * report["max_abs_logit_shift_of_codes"] + (
+        5e-4 if dtype == "float32" else 2.5e-2 * report["max_abs_logit_difference"] / report["max_difference_of_row_magnitude"])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_check_over_codes_still_finds_logits_that_are_off(dtype):
+    from types import SimpleNamespace
+
+    from metallix_b200.engine import cli
+    rows = torch.randn((3, 50), generator=torch.Generator().manual_seed(0)).cuda()
+    moved = torch.zeros_like(rows)
+    moved[1, 7] = 0.25      # what the codes move a logit by
+
+    def engine(logits):
+        return SimpleNamespace(step=lambda entries: logits, check=lambda: None, release=lambda name: None)
+    result = SimpleNamespace(input_ids=[1, 2], generated_ids=[3, 4, 5])
+    absolute, relative = cli.VERIFY_BOUNDS[dtype]
+    for times, within in ((0.0, True), (1.9, True), (2.2, False)):
+        off = rows.clone()
+        largest = rows[2].abs() if dtype == "float32" else rows[2].abs().amax()
+        off[2] += times * 0.25 + (absolute + relative * largest) * (1.0 if times > 2 else 0.0)
+        report = cli._verify_cache(engine(off), engine(rows), result, dtype, rows.cpu() - moved.cpu())
+        assert report["logits_within_bound"] is within and abs(report["max_abs_logit_shift_of_codes"] - 0.25) < 1e-6
+        assert cli._verify_cache(engine(off), engine(rows), result, dtype)["logits_within_bound"] is (times == 0.0)
