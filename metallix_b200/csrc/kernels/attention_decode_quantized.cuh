@@ -534,7 +534,7 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
           const float p = quant_exp2<T>(s[b][j] - m[j]);
           sum[j] += p;
           weight[b][j] = p * v_scale;
-          widest[j] = fmaxf(widest[j], weight[b][j]);
+          widest[j] = fmaxf(widest[j], fabsf(weight[b][j]));   // a pool of a caller's own may have scales of either sign
         }
       }
       if (!anew) {

@@ -971,3 +971,25 @@ def test_positions_beyond_the_table_are_reported(ops, head_dim, offset, last, op
     with pytest.raises(ops.KernelError, match="block-table"):
         ops.check_status("cuda")
     assert torch.equal(out, expect)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim", [64, 128, 256, 40])
+@pytest.mark.parametrize("signs", ["all", "keys", "mixed"])
+def test_scales_of_either_sign(ops, kind, dtype, head_dim, signs):
+    """A row stands for code * scale whatever the scale's sign: pools that a caller's own program made."""
+    lengths = [700, 40]
+    pages, table = spread_tables(lengths, 16, 1)
+    pool = random_pool(ops, kind, pages, 2, 16, head_dim, 2)
+    if signs == "mixed":
+        pool.scales.mul_(torch.where(torch.rand(pool.scales.shape, generator=torch.Generator().manual_seed(3)) > 0.5, 1.0, -1.0).cuda())
+    else:
+        pool.scales[:, :1 if signs == "keys" else 2].neg_()
+    q = torch.randn((2, 4, head_dim), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    out, positions, lists = torch.zeros_like(q), ints([n - 1 for n in lengths]), ints([0, 1])
+    ops.paged_attention_decode(q, pool, out, table, lists, lists, positions, 0.1, 700)
+    ops.check_status("cuda")
+    exact, bound = exact_decode(q, pool, table, [(0, 0), (1, 1)], positions, 0.1)
+    close_as_halves(out, exact, bound, dtype, 700)
