@@ -549,7 +549,8 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
         for (int offset = 4; offset < 32; offset <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
         top[j] = fmaxf(top[j] * carry[j], most);
         const float before = up[j];
-        up[j] = power_of_two(kQuantTop - max(static_cast<int>(__float_as_uint(top[j]) >> 23) - 127, -100));
+        // 2^125 at most, whose reciprocal __fdividef still gives (beyond 2^126 it gives 0)
+        up[j] = power_of_two(min(kQuantTop - (static_cast<int>(__float_as_uint(top[j]) >> 23) - 127), 125));
         // a quotient beyond float32 means that what was gathered is nothing on the new reference: carry is 0 then
         const float factor = carry[j] * fminf(up[j] / before, 0x1p127f);
         l[j] *= carry[j];

@@ -993,3 +993,28 @@ def test_scales_of_either_sign(ops, kind, dtype, head_dim, signs):
     ops.check_status("cuda")
     exact, bound = exact_decode(q, pool, table, [(0, 0), (1, 1)], positions, 0.1)
     close_as_halves(out, exact, bound, dtype, 700)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim", [64, 128, 256, 40])
+@pytest.mark.parametrize("size", [1e-32, 1e-34, 1e-36])
+@pytest.mark.parametrize("where", ["all", "later", "earlier"])
+def test_values_near_the_least_of_float32(ops, dtype, head_dim, size, where):
+    """Values of such a size throughout, and beside ordinary ones that come ahead of them or behind."""
+    lengths = [1500, 300]
+    pages, table = spread_tables(lengths, 16, 1)
+    pool = random_pool(ops, "fp8", pages, 2, 16, head_dim, 2)
+    for r, n in enumerate(lengths):
+        held = [int(p) for p in table[r, :-(-n // 16)]]
+        small = held if where == "all" else held[len(held) // 2:] if where == "later" else held[:len(held) // 2]
+        pool.scales[small, 1] *= size
+    q = torch.randn((2, 4, head_dim), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    out, positions, lists = torch.zeros_like(q), ints([n - 1 for n in lengths]), ints([0, 1])
+    ops.paged_attention_decode(q, pool, out, table, lists, lists, positions, 0.1, 1500)
+    ops.check_status("cuda")
+    exact, bound = exact_decode(q, pool, table, [(0, 0), (1, 1)], positions, 0.1)
+    # p_j scale_j and, times 2^125, its halves end at 2^-150 each: so much a key, times a code, over a sum of one or more
+    ends, off = 1500 * 448 * 2.0 ** -149, (out.double() - exact).abs()
+    # times 2^100, so that sizes count as in other tests
+    close_as_halves(torch.where(off <= ends, exact, out.double()) * 2.0 ** 100, exact * 2.0 ** 100, bound * 2.0 ** 100, dtype, 1500)
