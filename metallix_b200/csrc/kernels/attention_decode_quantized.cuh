@@ -86,7 +86,7 @@ quantized_decode_kernel(const QuantizedDecode a) {
 #pragma unroll
       for (int i = 0; i < VALUES; ++i) {
         const int d = lane + 32 * i;
-        k[i] = d < n ? code_value<KIND>(a.codes[k_row * n + d]) : 0.0f;
+        k[i] = d < n ? code_value<KIND>(a.codes[k_row * n + d]) * k_scale : 0.0f;   // q . code may leave float32 where the score does not
         v[i] = d < n ? code_value<KIND>(a.codes[v_row * n + d]) : 0.0f;
       }
 #pragma unroll
@@ -95,7 +95,7 @@ quantized_decode_kernel(const QuantizedDecode a) {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < VALUES; ++i) s = fmaf(q[h][i], k[i], s);
-        s = capped_score(warp_sum(s) * k_scale * a.scale, a.softcap);
+        s = capped_score(warp_sum(s) * a.scale, a.softcap);
         if (a.bias.table != nullptr) s += bias_at(a.bias.row(head0 + h), pos - key, a.bias.far);
         const float top = fmaxf(m[h], s), carry = expf(m[h] - top), p = expf(s - top);
         m[h] = top;
@@ -491,7 +491,8 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
       for (int b = 0; b < EIGHTS; ++b) {
         const float k_scale = scales[b * 8 + g];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) s[b][j] = (d[0][b / 2][2 * (b & 1) + j] + d[1][b / 2][2 * (b & 1) + j]) * to_score[j] * k_scale;
+        for (int j = 0; j < 2; ++j)   // the factors' product first: the sum times either of them may leave float32 where the score does not
+          s[b][j] = (d[0][b / 2][2 * (b & 1) + j] + d[1][b / 2][2 * (b & 1) + j]) * (to_score[j] * k_scale);
       }
     }
     if (scaled) {

@@ -1018,3 +1018,24 @@ def test_values_near_the_least_of_float32(ops, dtype, head_dim, size, where):
     ends, off = 1500 * 448 * 2.0 ** -149, (out.double() - exact).abs()
     # times 2^100, so that sizes count as in other tests
     close_as_halves(torch.where(off <= ends, exact, out.double()) * 2.0 ** 100, exact * 2.0 ** 100, bound * 2.0 ** 100, dtype, 1500)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("head_dim", [64, 128, 256, 40])
+@pytest.mark.parametrize("size", [1e32, 1e35, 3e37])
+def test_queries_near_the_largest_of_float32(ops, dtype, head_dim, size):
+    """Queries whose products with the codes pass float32's range while the scores do not, and the other way about."""
+    lengths = [700, 40]
+    pages, table = spread_tables(lengths, 16, 1)
+    plain = random_pool(ops, "fp8", pages, 2, 16, head_dim, 2)
+    q = torch.randn((2, 4, head_dim), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").clamp(-4, 4)
+    positions, lists = ints([n - 1 for n in lengths]), ints([0, 1])
+    for up in (size, 1.0 / size):
+        pool = ops.QuantizedPool(plain.codes, plain.scales.clone())
+        pool.scales[:, 0] /= up
+        large, out = (q * up).to(dtype), torch.zeros(q.shape, dtype=dtype, device="cuda")
+        ops.paged_attention_decode(large, pool, out, table, lists, lists, positions, 0.1, 700)
+        ops.check_status("cuda")
+        exact, bound = exact_decode(large, pool, table, [(0, 0), (1, 1)], positions, 0.1)
+        close_as_halves(out, exact, bound, dtype, 700)
