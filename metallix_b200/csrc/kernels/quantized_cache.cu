@@ -336,22 +336,22 @@ __global__ void __launch_bounds__(kReadThreads)
 read_cache_pieces_kernel(const __grid_constant__ ReadArgs a) {
   // No release ahead of the end: what follows has nothing to do before `out` is there.
   chain_wait();   // the codes are the work of kernels ahead
-  const int row = blockIdx.y, end = a.last[row], head_dim = a.head_dim, page_tokens = a.page_tokens;
+  // A last position beyond the table is cut to the first one there, whose page is found missing and reported.
+  const int end = static_cast<int>(min(static_cast<long long>(a.last[blockIdx.y]), static_cast<long long>(a.max_pages) * a.page_tokens));
+  const int row = blockIdx.y, head_dim = a.head_dim, page_tokens = a.page_tokens;
   if (end < 0) return;
   const KeyWalk walk = key_walk(min(first_visible_key(max(a.first[row], 0), a.window, a.chunk), end), end, a.keep, page_tokens);
   const int per_row = head_dim >> 4, rows = 2 * a.kv_heads * page_tokens, pieces = rows * per_row;
   const int per_page = (pieces + kReadPieces - 1) / kReadPieces;
   const int* table = a.block_tables + static_cast<size_t>(a.row_request[row]) * a.max_pages;
-  const int steps = min(walk.count, a.max_pages + 1);   // as many as the table has pages, and one that finds that there are no more
-  for (int item = blockIdx.x; item < steps * per_page; item += gridDim.x) {
+  for (int item = blockIdx.x; item < walk.count * per_page; item += gridDim.x) {
     const int step = item / per_page, slot = walk.tile(step), piece0 = (item - step * per_page) * kReadPieces;
     const int page = slot < a.max_pages ? table[slot] : -1;
     if (page < 0 || page >= a.num_pages) {
       if (threadIdx.x == 0) atomicOr(a.status, kStatusBadPage);
-      if (slot >= a.max_pages) break;   // `last` lies beyond the table, and so do all further steps
       continue;
     }
-    const int seen = min(end - slot * page_tokens, page_tokens - 1) + 1;   // rows of the page up to the last position
+    const int seen = end - slot * page_tokens + 1;   // rows of the page up to the last position
     const size_t base = static_cast<size_t>(page) * rows;
     const uint4* src = reinterpret_cast<const uint4*>(a.codes + base * head_dim);
     uint4 held[kReadDepth];
