@@ -155,7 +155,7 @@ quantized_decode_kernel(const QuantizedDecode a) {
 // its own by TMA, one box per page and plane with the swizzle that lets its lanes
 // read them without bank conflicts. (With copies of 16 bytes a lane by cp.async
 // 8 requests over 32,000 positions took 113 to 130 us, whatever depth and number
-// of blocks an SM was tried; by TMA 87.6 when they were changed.)
+// of blocks an SM was tried; by TMA 90.)
 // What a lane reads is chosen so that bytes need no transposing:
 //   K: lane (g, t) = (lane / 4, lane % 4) reads the 16-byte chunks 2t, 2t + 1 of the
 //      key g of eight (heads of 64: chunk t). Word w of a chunk of the keys g and
@@ -167,7 +167,9 @@ quantized_decode_kernel(const QuantizedDecode a) {
 //      movmatrix. No row of either product is wasted.
 //
 // float32 queries are two halves each, 22 bits and the sign of what is left; so
-// are the weights: a second product for either.
+// are the weights: a second product for either. For bfloat16 queries, which one
+// half holds whole, the weights are one half, eleven bits, three more than the
+// output's; the sum that they are divided by takes them unrounded.
 template <int HD> struct QuantTile {
   static constexpr int kKeys = HD == 256 ? 16 : 32;            // of a stage
   static constexpr int kBlocks8 = kKeys / 8;                   // eights of keys
@@ -250,7 +252,8 @@ __device__ __forceinline__ float quant_peer(const float* mine, int rank) {
   return value;
 }
 
-// Blocks resident on an SM: what the ring and the registers leave room for.
+// Blocks resident on an SM: what the ring and the registers leave room for. Heads of 64 (bfloat16) have room for a fourth,
+// which is worth little: 8 requests of 32,000 positions 61 us with three and 58 with four, 61 ragged ones 55 and 55.
 template <typename T, int HD> struct QuantBlocks {
   static constexpr int value = HD == 256 ? (std::is_same<T, float>::value ? 1 : 2) : 3;
 };
@@ -671,8 +674,12 @@ static bool quantized_mma_takes(const QuantizedDecode& a) {
 
 // How many blocks a (token, key/value head) pair gets of the tensor-core kernel, `tiles` being the most that one has and
 // `resident` how many blocks the GPU holds. Where that leaves blocks eight tiles or more, two rounds of blocks: the contexts of
-// a batch differ, and blocks of the longest would be alone for half the time (16 requests of up to 32,000 positions: 122 us
-// in one round, 92 in two; 8 of 32,000 each: 88 and 92). Else one round, and a tile or two a block where there are few.
+// a batch differ, and blocks of the longest would be alone for half the time. With 8 key/value heads and contexts spread
+// evenly up to 36,000 positions (heads of 128, four to a key/value head; us in one round and in two): 4 requests 43 and 40,
+// 8 requests 73 and 60, 16 requests 135 and 102; contexts of one length pay for it: 8 of 32,000 86 and 89, 16 of 8,000 47
+// and 52. From four tiles a block on, 8 of 8,000 would go from 28 to 31, and few ragged requests (3 to 16 with 1 to 8 key/value
+// heads) gain or lose 1 us or less.
+// Else one round, and two tiles a block from 32 tiles on (1 of 8,000: 11.2, with one tile a block 12.6).
 static int quantized_slots(int pairs, int tiles, int resident) {
   const int twice = pairs <= resident ? 2 * resident / pairs : (2 * resident + pairs / 2) / pairs;
   if (pairs > 1 && twice > 1 && tiles >= 8 * twice) return twice;
@@ -712,7 +719,8 @@ static cudaError_t launch_quantized_decode(QuantizedDecode args, int kind, int r
     const int resident = 148 * (args.head_dim == 256 ? QuantBlocks<T, 256>::value : QuantBlocks<T, 128>::value);
     int count = quantized_slots(pairs, tiles, resident);
     // Few tiles over a few more blocks than a cluster has: the launch and the trip through memory that the merge kernel
-    // costs are worth more than the blocks.
+    // costs are worth more than the blocks (4 requests of 2,048 positions 8.2 us, else 10.4; 4 of 5,000 14.0 and 14.9; but 1
+    // of 4,096 9.6 and 8.5). Not with longer contexts: 1 of 8,000 would go from 11.2 to 13.9.
     if (fusable && count > kQuantCluster && tiles <= 6 * kQuantCluster && kQuantCluster * pairs <= resident) count = kQuantCluster;
     // Clusters only where all blocks are resident at once: in further rounds a cluster waits for as many places side by side
     // (37 requests of 7,000 positions in three blocks a pair: 115 us as clusters, 92 without).

@@ -103,8 +103,9 @@ template <int KIND> __device__ __forceinline__ uint32_t round_to_codes(const flo
 }
 
 // Four values' codes as the bytes of a word. The product by the reciprocal is within 2^-23 of the quotient, so if both ends
-// of the numbers within 2^-21 of it have one code that is the quotient's; else (one value in 10^5, and rows whose scale is a
-// power of two) the quotient is rounded to odd first. Five instructions a value instead of fourteen.
+// of the numbers within 2^-21 of it have one code that is the quotient's; else (of e4m3 codes one value in 10^5, of whole
+// numbers |code| x 2^-20, 12 in 10^5 at most; more where the scale is a power of two; and rows whose scale lies beyond
+// 2^-60 ... 2^60) the quotient is rounded to odd first. Five instructions a value instead of fourteen.
 template <int KIND> __device__ __forceinline__ uint32_t four_codes(const float* x, const RowScale& r) {
   if (r.inverse == 0.0f) return 0u;   // a row of zeros, or one that is not finite
   float below[4], beyond[4];
