@@ -24,6 +24,14 @@ constexpr int kDecodeThreads = 128;
 constexpr unsigned kDecodeBlocksAtOnce = 444;   // blocks of the bfloat16 kernels a B200 holds at once: three an SM
 constexpr float kDecodeMinusHuge = -1.0e30f;
 
+// Where entry `i` of a row's block table lies, or, for a row that the tables do not have (padding rows may name any), their
+// first entry: for a look ahead of the token, which says whether the row is padding. (To wait for the token, or to branch on
+// the row, costs a decode step some 0.4%.)
+__device__ __forceinline__ size_t table_entry(int row, int i, int max_pages, int table_rows) {
+  const unsigned long long at = static_cast<unsigned long long>(static_cast<unsigned>(row)) * max_pages + i;
+  return at < static_cast<unsigned long long>(table_rows) * max_pages ? at : 0;
+}
+
 template <typename T> struct Vec16;  // 16 bytes of T
 template <> struct Vec16<float> {
   static constexpr int kElems = 4;
@@ -489,7 +497,7 @@ template <int HD, bool BIASED>
 __global__ void __launch_bounds__(kDecodeThreads)
 paged_attention_decode_tma_kernel(const __grid_constant__ CUtensorMap map_cache, const __nv_bfloat16* __restrict__ q,
                                   float* __restrict__ partial, const int* __restrict__ block_tables,
-                                  int max_pages, const int* __restrict__ row_token,
+                                  int max_pages, int table_rows, const int* __restrict__ row_token,
                                   const int* __restrict__ row_request, const int* __restrict__ positions,
                                   int heads, int kv_heads, int page_tokens, int num_pages, int max_splits,
                                   int window, int chunk, int keep, float scale, float softcap, ScoreBias bias, int* status) {
@@ -526,13 +534,13 @@ paged_attention_decode_tma_kernel(const __grid_constant__ CUtensorMap map_cache,
   // the page.
   const int token = row_token[row];
   const int table_row = row_request[row];
-  if (token < 0) {   // a padding row: its row_request may be anything
-    chain_wait();
-    return;
-  }
   int page = 0;
   if (fetcher && page_key / page_tokens < max_pages)
-    page = block_tables[static_cast<size_t>(table_row) * max_pages + page_key / page_tokens];
+    page = block_tables[table_entry(table_row, page_key / page_tokens, max_pages, table_rows)];
+  if (token < 0) {
+    chain_wait();   // as above
+    return;
+  }
   const int pos = positions[token];
   const int group = heads / kv_heads;  // <= 8
   const int first_key = first_visible_key(pos, window, chunk);
@@ -715,7 +723,7 @@ template <int HD, bool BIASED>
 __global__ void __launch_bounds__(kDecodeThreads, 3)
 paged_attention_decode_resident_kernel(const __grid_constant__ CUtensorMap map_cache, const __nv_bfloat16* __restrict__ q,
                                        float* __restrict__ partial, const int* __restrict__ block_tables,
-                                       int max_pages, const int* __restrict__ row_token,
+                                       int max_pages, int table_rows, const int* __restrict__ row_token,
                                        const int* __restrict__ row_request, const int* __restrict__ positions,
                                        int heads, int kv_heads, int page_tokens, int num_pages, int max_splits,
                                        int window, int chunk, int keep, float scale, float softcap, ScoreBias bias, int* status) {
@@ -741,15 +749,15 @@ paged_attention_decode_resident_kernel(const __grid_constant__ CUtensorMap map_c
   const int which = tid / (pages * HALVES), slot = (tid / HALVES) % pages, half = tid % HALVES;
   const int token = row_token[row];
   const int table_row = row_request[row];
-  if (token < 0) {   // a padding row: its row_request may be anything
-    chain_wait();
-    return;
-  }
   const int* table = block_tables + static_cast<size_t>(table_row) * max_pages;
   // The page of this block's first tile is asked for together with the
   // position, on the guess that neither a window nor a chunk has moved the first tile.
   int page = 0;
-  if (fetcher && rank * pages + slot < max_pages) page = table[rank * pages + slot];
+  if (fetcher && rank * pages + slot < max_pages) page = block_tables[table_entry(table_row, rank * pages + slot, max_pages, table_rows)];
+  if (token < 0) {   // a padding row
+    chain_wait();
+    return;
+  }
   const int pos = positions[token];
   const int group = heads / kv_heads;  // <= 8
   const int first_key = first_visible_key(pos, window, chunk);
@@ -1077,7 +1085,7 @@ struct DecodeProject {
 
 template <typename T, int HD, int G>
 static int launch_decode(const void* q, const void* cache, void* out, float* partial,
-                         const int* block_tables, int max_pages, const int* row_token,
+                         const int* block_tables, int max_pages, int table_rows, const int* row_token,
                          const int* row_request, const int* positions, int rows, int heads,
                          int kv_heads, int page_tokens, int num_pages, int max_splits, int window, int chunk, int keep,
                          float scale, int* status, cudaStream_t stream, DecodeProject project = DecodeProject()) {
@@ -1111,7 +1119,7 @@ constexpr int kLongSplits = 32;            // tiles from which on contexts are l
 
 template <int HD>
 static int launch_decode_mma(const void* q, const void* cache, void* out, float* partial,
-                             const int* block_tables, int max_pages, const int* row_token,
+                             const int* block_tables, int max_pages, int table_rows, const int* row_token,
                              const int* row_request, const int* positions, int rows, int heads,
                              int kv_heads, int page_tokens, int num_pages, int max_splits, int window, int chunk, int keep,
                              float scale, int* status, cudaStream_t stream, DecodeProject project = DecodeProject()) {
@@ -1167,7 +1175,7 @@ static int launch_decode_mma(const void* q, const void* cache, void* out, float*
       cudaError_t attribute = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
       if (attribute != cudaSuccess) return static_cast<int>(attribute);
       e = launch_chained(kernel, dim3(slots, kv_heads, rows), dim3(kDecodeThreads), shared, stream, map_cache,
-                         static_cast<const __nv_bfloat16*>(q), partial, block_tables, max_pages, row_token, row_request,
+                         static_cast<const __nv_bfloat16*>(q), partial, block_tables, max_pages, table_rows, row_token, row_request,
                          positions, heads, kv_heads, page_tokens, num_pages, max_splits, window, chunk, keep, scale, project.softcap, project.bias, status);
       if (e != cudaSuccess) return static_cast<int>(e);
       return finish(slots);
@@ -1177,7 +1185,7 @@ static int launch_decode_mma(const void* q, const void* cache, void* out, float*
     cudaError_t attribute = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
     if (attribute != cudaSuccess) return static_cast<int>(attribute);
     e = launch_chained(kernel, grid, dim3(kDecodeThreads), shared, stream, map_cache,
-                       static_cast<const __nv_bfloat16*>(q), partial, block_tables, max_pages, row_token, row_request,
+                       static_cast<const __nv_bfloat16*>(q), partial, block_tables, max_pages, table_rows, row_token, row_request,
                        positions, heads, kv_heads, page_tokens, num_pages, max_splits, window, chunk, keep, scale, project.softcap, project.bias, status);
   } else {
     const int shared = 2 * kSplitKeys * (HD * 2 + 16);
@@ -1221,10 +1229,11 @@ MXB_API int mxb_set_decode_resident_blocks(int blocks, int many) {
 }
 
 // partial: float32 scratch of rows * heads * max_splits * (head_dim + 2) values.
-// rows of row_token that are negative are padding. max_splits must cover the
+// rows of row_token that are negative are padding; their row_request does not matter.
+// table_rows: how many rows the block tables have. max_splits must cover the
 // longest context: ceil(longest / 128).
 MXB_API int mxb_paged_attention_decode(const void* q, const void* cache, void* out, float* partial,
-                                       const int* block_tables, int max_pages, const int* row_token,
+                                       const int* block_tables, int max_pages, int table_rows, const int* row_token,
                                        const int* row_request, const int* positions, int rows,
                                        int heads, int kv_heads, int head_dim, int page_tokens,
                                        int num_pages, int max_splits, int window, int chunk, int keep, float scale,
@@ -1232,6 +1241,7 @@ MXB_API int mxb_paged_attention_decode(const void* q, const void* cache, void* o
                                        float sink_score, const float* sink_heads, const float* bias_table, int bias_far,
                                        int* status, cudaStream_t stream) {
   if (rows <= 0) return 0;
+  if (table_rows <= 0) table_rows = max_pages = 0;   // no tables: nothing is looked up
   if (bias_table != nullptr && bias_far < 0) return static_cast<int>(cudaErrorInvalidValue);
   if (!mxb_paged_attention_decode_supported(head_dim, heads, kv_heads, dtype) || max_splits <= 0)
     return static_cast<int>(cudaErrorInvalidValue);
@@ -1244,7 +1254,7 @@ MXB_API int mxb_paged_attention_decode(const void* q, const void* cache, void* o
   project.sink_score = sink_score;
   project.sink_heads = sink_heads;
   project.bias = ScoreBias{bias_table, bias_far};
-#define ARGS q, cache, out, partial, block_tables, max_pages, row_token, row_request, positions, rows, \
+#define ARGS q, cache, out, partial, block_tables, max_pages, table_rows, row_token, row_request, positions, rows, \
              heads, kv_heads, page_tokens, num_pages, max_splits, window, chunk, keep, scale, status, stream, project
 #define BY_GROUP(T, HD)                                        \
   if (group == 1) return launch_decode<T, HD, 1>(ARGS);        \
@@ -1277,7 +1287,7 @@ MXB_API int mxb_paged_attention_decode_project_supported(int head_dim, int heads
 // in float32, [heads, tokens, hidden]; their sum over h is the projected
 // output. Tokens that no row names give zeros. w: [hidden, heads * head_dim].
 MXB_API int mxb_paged_attention_decode_project(const void* q, const void* cache, float* partial,
-                                               const int* block_tables, int max_pages, const int* row_token,
+                                               const int* block_tables, int max_pages, int table_rows, const int* row_token,
                                                const int* row_request, const int* positions, int rows, int tokens,
                                                int heads, int kv_heads, int head_dim, int page_tokens, int num_pages,
                                                int max_splits, int window, int chunk, int keep, float scale, const void* w, long long ldw,
@@ -1286,6 +1296,7 @@ MXB_API int mxb_paged_attention_decode_project(const void* q, const void* cache,
                                                const float* bias_table, int bias_far, int* status, cudaStream_t stream) {
   if (bias_table != nullptr && bias_far < 0) return static_cast<int>(cudaErrorInvalidValue);
   if (rows <= 0 || hidden <= 0 || max_splits <= 0) return static_cast<int>(cudaErrorInvalidValue);
+  if (table_rows <= 0) table_rows = max_pages = 0;   // no tables: nothing is looked up
   if (!mxb_paged_attention_decode_project_supported(head_dim, heads, kv_heads, kBF16, tokens, w, ldw))
     return static_cast<int>(cudaErrorInvalidValue);
   DecodeProject project;
@@ -1302,7 +1313,7 @@ MXB_API int mxb_paged_attention_decode_project(const void* q, const void* cache,
   project.sink_heads = sink_heads;
   project.bias = ScoreBias{bias_table, bias_far};
   void* out = nullptr;
-#define ARGS q, cache, out, partial, block_tables, max_pages, row_token, row_request, positions, rows, \
+#define ARGS q, cache, out, partial, block_tables, max_pages, table_rows, row_token, row_request, positions, rows, \
              heads, kv_heads, page_tokens, num_pages, max_splits, window, chunk, keep, scale, status, stream, project
   return head_dim == 64 ? launch_decode_mma<64>(ARGS) : launch_decode_mma<128>(ARGS);
 #undef ARGS
@@ -1327,7 +1338,7 @@ struct QuantizedDecodeCall {
   const void* gate;
   const float *sink_heads, *bias_table;
   int* status;
-  long long kind, dtype, max_pages, rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, max_splits, window, chunk, keep,
+  long long kind, dtype, max_pages, table_rows, rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, max_splits, window, chunk, keep,
       ldw, hidden, gate_stride, has_sink, bias_far, settled;
   double scale, softcap, sink_score;
 };
@@ -1362,8 +1373,9 @@ MXB_API int mxb_paged_attention_decode_quantized(const void* call, int bytes, cu
   int page_shift = 0;
   while ((1LL << page_shift) < c.page_tokens) ++page_shift;
   if ((1LL << page_shift) != c.page_tokens) page_shift = -1;
+  const bool tables = c.table_rows > 0;   // none: nothing is looked up
   const QuantizedDecode args = {c.q, static_cast<const uint8_t*>(c.codes), c.scales, c.partial, c.block_tables,
-                                static_cast<int>(c.max_pages), c.row_token, c.row_request, c.positions, heads, kv_heads, head_dim,
+                                tables ? static_cast<int>(c.max_pages) : 0, tables ? static_cast<int>(c.table_rows) : 0, c.row_token, c.row_request, c.positions, heads, kv_heads, head_dim,
                                 static_cast<int>(c.page_tokens), static_cast<int>(c.num_pages), window, chunk, keep,
                                 static_cast<float>(c.scale), static_cast<float>(c.softcap),
                                 ScoreBias{c.bias_table, static_cast<int>(c.bias_far)}, heads / kv_heads, page_shift, static_cast<int>(c.settled), c.status,
@@ -1453,7 +1465,8 @@ MXB_API int mxb_paged_attention_decode_noalloc(const void* q, const void* cache,
   float* scratch = nullptr;
   const cudaError_t e = noalloc_scratch_address(&scratch);
   if (e != cudaSuccess) return static_cast<int>(e);
-  return mxb_paged_attention_decode(q, cache, out, scratch, block_tables, max_pages, row_token,
+  // how many rows the tables have is not known here: a padding row's row_request is negative or one of them
+  return mxb_paged_attention_decode(q, cache, out, scratch, block_tables, max_pages, 0x7fffffff, row_token,
                                     row_request, positions, rows, heads, kv_heads, head_dim, page_tokens,
                                     num_pages, splits, window, 0, 0, scale, dtype, nullptr, 0, 0.0f, 0, 0.0f, nullptr, nullptr, 0, status, stream);
 }

@@ -28,7 +28,8 @@
 // scratch pointer: q and out [tokens, heads, head_dim], cache
 // [pages, 2, kv_heads, page_tokens, head_dim], block_tables
 // [requests, max_pages] int32, row_token / row_request [rows] int32 (a
-// negative row_token is a padding row), positions [tokens] int32; dtype 0 is
+// negative row_token is a padding row, whose row_request is negative too or
+// a row of block_tables), positions [tokens] int32; dtype 0 is
 // float32, 1 is bfloat16; status is a device int32 the kernels OR error bits
 // into. Returns a cudaError_t value, 0 on success.
 #pragma once

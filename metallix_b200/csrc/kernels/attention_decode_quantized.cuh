@@ -21,7 +21,7 @@ struct QuantizedDecode {
   const float* scales;
   float* partial;                // [rows, heads, slots, head_dim + 2]
   const int* block_tables;
-  int max_pages;
+  int max_pages, table_rows;     // what the block tables have of columns and rows
   const int *row_token, *row_request, *positions;
   int heads, kv_heads, head_dim, page_tokens, num_pages, window, chunk, keep;
   float scale, softcap;
@@ -293,13 +293,16 @@ quantized_decode_mma_kernel(const __grid_constant__ CUtensorMap map_codes, const
     barrier_init_fence();
   }
   __syncwarp();
-  if (token < 0) {   // a padding row: its row_request may be anything
-    chain_wait();    // a launch that ends ahead of the one before it lets what follows start too early
+  auto guess_at = [&](int key) {   // a padding row's request may be no row of the tables
+    return (key >> shift) < a.max_pages ? a.block_tables[table_entry(request, key >> shift, a.max_pages, a.table_rows)] : -1;
+  };
+  int box_page = guess_at(rank * kSplitKeys + warp * 32 + box_key), scale_page = guess_at(rank * kSplitKeys + warp * 32 + scale_key);
+  if (token < 0) {
+    chain_wait();   // a launch that ends ahead of the one before it lets what follows start too early
     return;
   }
   const int* table = a.block_tables + static_cast<size_t>(request) * a.max_pages;
   auto page_at = [&](int key) { return (key >> shift) < a.max_pages ? table[key >> shift] : -1; };
-  int box_page = page_at(rank * kSplitKeys + warp * 32 + box_key), scale_page = page_at(rank * kSplitKeys + warp * 32 + scale_key);
   const int pos = a.positions[token];
   const int live = min(group - part * 8, 8), head0 = kv * group + part * 8;   // this block's query heads
   const int first_key = first_visible_key(pos, a.window, a.chunk);

@@ -90,7 +90,7 @@ _SIGNATURES = {
                          _I, _P, _P],
     "mxb_rotate_into": [_P, _L, _I, _I, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _I, _P, _P],
     "mxb_plain_activation": [_P, _P, _L, _I, _I, _P],
-    "mxb_paged_attention_decode": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
+    "mxb_paged_attention_decode": [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
                                    _F, _I, _P, _L, _F, _I, _F, _P, _P, _I, _P, _P],
     "mxb_paged_attention_decode_quantized": [_C, _I, _P],
     "mxb_store_quantized": [_C, _I, _P],
@@ -100,7 +100,7 @@ _SIGNATURES = {
     "mxb_softcap": [_P, _F, _L, _P],
     "mxb_paged_attention_decode_supported": [_I, _I, _I, _I],
     "mxb_paged_attention_decode_project_supported": [_I, _I, _I, _I, _I, _P, _L],
-    "mxb_paged_attention_decode_project": [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
+    "mxb_paged_attention_decode_project": [_P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I,
                                            _F, _P, _L, _I, _P, _P, _L, _F, _I, _F, _P, _P, _I, _P, _P],
     "mxb_paged_attention_split_keys": [],
     "mxb_set_decode_resident_blocks": [_I, _I],
@@ -1385,7 +1385,7 @@ def _ints_on(device: int, dims: int, *tensors) -> bool:
 # The calls' fields, in the order of the structs of the same names in csrc/kernels: pointers and whole numbers, then doubles.
 _READ_CALL = struct.Struct("=19q")
 _STORE_CALL = struct.Struct("=31qd")
-_QUANTIZED_DECODE_CALL = struct.Struct("=35q3d")
+_QUANTIZED_DECODE_CALL = struct.Struct("=36q3d")
 
 
 def read_cache(pool: QuantizedPool, out: torch.Tensor, block_tables: torch.Tensor, row_request: torch.Tensor,
@@ -1871,7 +1871,7 @@ def _decode_quantized(q: torch.Tensor, pool: QuantizedPool, out: Optional[torch.
         0 if partial is None else partial.data_ptr(), block_tables.data_ptr(), row_token.data_ptr(), row_request.data_ptr(),
         positions.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if summands is None else summands.data_ptr(),
         0 if gate is None else gate.data_ptr(), sink_heads or 0, bias_table or 0, _status_pointer(device), pool.kind, _CODES[dtype],
-        block_tables.shape[1], rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits, _reach(window),
+        block_tables.shape[1], block_tables.shape[0], rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits, _reach(window),
         _reach(chunk), min(_kept(keep), _FAR) if keep else 0, ldw, hidden, gate_stride, has_sink, bias_far, 1 if settled else 0, scale, softcap, sink_score]
     call, stream = _QUANTIZED_DECODE_CALL.pack(*fields), _stream()
     entry = _fn("mxb_paged_attention_decode_quantized")
@@ -1948,7 +1948,7 @@ def paged_attention_decode(q: torch.Tensor, cache, out: torch.Tensor,
     _need(partial.numel() >= need, f"partial holds {partial.numel()} values, {need} are needed")
     gate_stride = _gate_stride(gate, q)
     _call("mxb_paged_attention_decode", q.data_ptr(), cache.data_ptr(), out.data_ptr(), partial.data_ptr(),
-          block_tables.data_ptr(), block_tables.shape[1], row_token.data_ptr(), row_request.data_ptr(),
+          block_tables.data_ptr(), block_tables.shape[1], block_tables.shape[0], row_token.data_ptr(), row_request.data_ptr(),
           positions.data_ptr(), rows, heads, kv_heads, head_dim, page_tokens, num_pages, splits,
           int(window or 0), int(chunk or 0), _kept(keep), float(scale), _CODES[dtype], _ptr(gate), gate_stride, float(softcap),
           *_sink(sink, heads), *_score_bias(bias, heads), status_word(q.device).data_ptr(), _stream())
@@ -2014,7 +2014,7 @@ def paged_attention_decode_project(q: torch.Tensor, cache, block_tables: torch.T
     summands = torch.empty((heads, tokens, hidden), dtype=torch.float32, device=q.device)
     gate_stride = _gate_stride(gate, q)
     _call("mxb_paged_attention_decode_project", q.data_ptr(), cache.data_ptr(), partial.data_ptr(),
-          block_tables.data_ptr(), block_tables.shape[1], row_token.data_ptr(), row_request.data_ptr(),
+          block_tables.data_ptr(), block_tables.shape[1], block_tables.shape[0], row_token.data_ptr(), row_request.data_ptr(),
           positions.data_ptr(), rows, tokens, heads, kv_heads, head_dim, page_tokens, num_pages, splits,
           int(window or 0), int(chunk or 0), _kept(keep), float(scale), weight.data_ptr(), weight.stride(0), hidden, summands.data_ptr(),
           _ptr(gate), gate_stride, float(softcap), *_sink(sink, heads), *_score_bias(bias, heads),

@@ -1039,3 +1039,22 @@ def test_queries_near_the_largest_of_float32(ops, dtype, head_dim, size):
         ops.check_status("cuda")
         exact, bound = exact_decode(large, pool, table, [(0, 0), (1, 1)], positions, 0.1)
         close_as_halves(out, exact, bound, dtype, 700)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", None])
+@pytest.mark.parametrize("head_dim,page,width", [(128, 16, 40), (64, 8, 3), (128, 16, 0), (256, 16, 5)])
+def test_padding_alone_over_tables_without_rows(ops, kind, head_dim, page, width):
+    pool = random_pool(ops, "fp8", 4, 2, page, head_dim, 1)
+    dtype = BF16 if kind or head_dim < 256 else F32
+    if kind is None:
+        if not ops.decode_attention_supported(head_dim, 4, 2, dtype):
+            pytest.skip("the split-key kernel does not take this layout")
+        pool = values_of(pool).to(dtype)
+    q = torch.zeros((2, 4, head_dim), dtype=dtype, device="cuda")
+    out = torch.full_like(q, 3.0)
+    table = torch.empty((0, width), dtype=torch.int32, device="cuda")
+    for longest in (60, 6000):
+        ops.paged_attention_decode(q, pool, out, table, ints([-1, -1, -3]), ints([-1, 7, 2 ** 31 - 1]), ints([0, 0]), 0.1, longest)
+    ops.check_status("cuda")
+    assert out.eq(3.0).all()
